@@ -1,0 +1,296 @@
+"""Cases of the layer-chain operators: layer normalisation, dropout and the label embedding.
+
+The operators (``mmvae_amd.ops``) serve the hidden layers of the count VAEs: a Linear's output is
+normalised, dropped out and passed on; a cell's label (batch, donor) or its expressed genes are looked
+up in a table.  ``run`` makes one pass through one operator: with ``own`` false in elementary torch
+operations, with ``own`` true through the framework.  ``exact`` states the definitions in 64 bits.
+
+Layer norm of a row x of N values, with weight w and bias b:
+    mu = mean x,  r = 1 / sqrt(mean (x - mu)^2 + eps),  xh = (x - mu) r,  y = (xh w + b) m
+    du = dy m,  db = sum_rows du,  dw = sum_rows du xh,  g = du w,  dx = r (g - mean g - xh mean(g xh))
+with the dropout factor m in {0, s} (1 without dropout).
+Dropout of x [M, N] with probability p: thr = floor(65536 p + 1/2), s = 65536 / (65536 - thr).  The 16
+random bits of (row, col) are half col % 8 of Philox4x32-10's four words at the counter (col / 8, row,
+step, step >> 32) under the key (seed, seed >> 32); an element is kept where they are >= thr.
+Embedding: y[t] = s E[id[t]], a zero row for an id outside [0, V); dE[v] = s sum of dy[t] over id[t] = v.
+"""
+import math
+import os
+import sys
+
+import numpy as np
+import torch
+
+own = False
+
+_TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+_SIZE = {"f32": 4, "bf16": 2, "f16": 2}
+_EPS = 1e-5
+
+
+def _ops():
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    path = os.path.join(root, "mm-vae_amd", "py")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from mmvae_amd import ops
+    return ops
+
+
+# ---- cases -----------------------------------------------------------------------------------
+def listed():
+    return [
+        # one cell through a hidden layer of a trained encoder: only the latency counts
+        {"name": "norm one cell", "op": "norm", "M": 1, "N": 128, "type": "f32", "pad": 0, "train": False, "p": 0.0},
+        # the command line's defaults: a batch of 100 cells, a hidden layer of 48
+        {"name": "norm batch 100", "op": "norm", "M": 100, "N": 48, "type": "f32", "pad": 0, "train": True, "p": 0.0},
+        # a training batch of 4096 cells through a hidden layer of 128, with dropout
+        {"name": "norm dropout hidden", "op": "norm", "M": 4096, "N": 128, "type": "f32", "pad": 0, "train": True, "p": 0.1},
+        # odd width, rows inside a wider buffer
+        {"name": "norm odd strided", "op": "norm", "M": 777, "N": 1001, "type": "f16", "pad": 6, "train": True, "p": 0.0},
+        # a wide hidden layer over a large global batch, norm and dropout in one pass
+        {"name": "norm dropout wide", "op": "norm", "M": 32768, "N": 1024, "type": "bf16", "pad": 0, "train": True, "p": 0.2},
+        # expression rows normalised over all 20,000 genes
+        {"name": "norm genes", "op": "norm", "M": 4096, "N": 20000, "type": "bf16", "pad": 0, "train": True, "p": 0.0},
+        # dropout alone on a small batch
+        {"name": "dropout batch 100", "op": "dropout", "M": 100, "N": 128, "type": "f32", "p": 0.1},
+        # dropout of the input expression rows
+        {"name": "dropout genes", "op": "dropout", "M": 4096, "N": 20000, "type": "bf16", "p": 0.2},
+        # one cell's label
+        {"name": "embed one label", "op": "embed", "T": 1, "V": 30, "N": 64, "type": "f32", "train": False, "skew": False},
+        # a training batch's batch / donor labels: few rows with many tokens each
+        {"name": "embed labels", "op": "embed", "T": 4096, "V": 12, "N": 128, "type": "f32", "train": True, "skew": False},
+        # 64 expressed genes a cell, a table over 20,000 genes, a few genes in nearly every cell
+        {"name": "embed genes", "op": "embed", "T": 262144, "V": 20000, "N": 128, "type": "bf16", "train": True, "skew": True},
+        # odd sizes, and wide rows in a large table
+        {"name": "embed odd wide", "op": "embed", "T": 50001, "V": 30011, "N": 517, "type": "f16", "train": True, "skew": True},
+    ]
+
+
+def _between(rng, lo, hi):
+    """A whole number in [lo, hi], spread over its logarithm."""
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    kind = rng.choice(("norm", "norm", "norm", "dropout", "embed", "embed"))
+    typ = rng.choice(("f32", "bf16", "f16"))
+    most = 4096 * 20000 * 2 // _SIZE[typ]  # elements: no more bytes than the largest listed case
+    if kind == "embed":
+        n = _between(rng, 8, 1024)
+        t = _between(rng, 1, min(262144, most // (2 * n)))
+        return {"op": "embed", "T": t, "V": _between(rng, 2, 30000), "N": n, "type": typ,
+                "train": rng.random() < 0.75, "skew": rng.random() < 0.5}
+    n = _between(rng, 8, 30000)
+    m = _between(rng, 1, min(65536, most // n))
+    if kind == "dropout":
+        return {"op": "dropout", "M": m, "N": n, "type": typ, "p": round(rng.uniform(0.05, 0.6), 3)}
+    return {"op": "norm", "M": m, "N": n, "type": typ, "pad": rng.choice((0, 0, 0, 1, 8)),
+            "train": rng.random() < 0.75, "p": rng.choice((0.0, 0.0, round(rng.uniform(0.05, 0.6), 3)))}
+
+
+# ---- inputs ----------------------------------------------------------------------------------
+def _normal(g, shape, typ, pad=0):
+    """Standard normal values; pad > 0: the rows of a wider buffer."""
+    x = torch.randn(shape[0], shape[1] + pad, generator=g, device="cuda").to(_TYPES[typ])
+    return x[:, :shape[1]]
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1000003 * seed + 17)
+    s = dict(case)
+    s["seed"], s["step"] = seed * 7919 + 13, seed + 5
+    typ = case["type"]
+    if case["op"] == "embed":
+        t, v, n = case["T"], case["V"], case["N"]
+        s["table"] = _normal(g, (v, n), typ)
+        if case["skew"]:  # frequency of a row about 1 / rank, the ranks in no order
+            u = torch.rand(t, generator=g, device="cuda", dtype=torch.float64)
+            rank = (torch.exp(u * math.log(v + 1)) - 1).long().clamp_(0, v - 1)
+            s["ids"] = torch.randperm(v, generator=g, device="cuda")[rank]
+        else:
+            s["ids"] = torch.randint(0, v, (t,), generator=g, device="cuda")
+        if t >= 64:  # cells without a label
+            s["ids"][torch.randint(0, t, (t // 64,), generator=g, device="cuda")] = -1
+        s["scale"] = math.sqrt(n)
+        if case["train"]:
+            s["dy"] = _normal(g, (t, n), typ)
+        return s
+    m, n = case["M"], case["N"]
+    if case["op"] == "dropout":
+        s["x"] = _normal(g, (m, n), typ)
+        s["dy"] = _normal(g, (m, n), typ)
+        return s
+    # a Linear's output: every row has a mean and a spread of its own
+    centre = torch.randn(m, 1, generator=g, device="cuda")
+    spread = 0.5 + torch.rand(m, 1, generator=g, device="cuda")
+    x = torch.randn(m, n + case["pad"], generator=g, device="cuda").mul_(spread).add_(centre)
+    s["x"] = x.to(_TYPES[typ])[:, :n]
+    s["w"] = 1 + 0.2 * torch.randn(n, generator=g, device="cuda")
+    s["b"] = 0.2 * torch.randn(n, generator=g, device="cuda")
+    if case["train"]:
+        s["dy"] = _normal(g, (m, n), typ)
+    return s
+
+
+# ---- one pass --------------------------------------------------------------------------------
+def run(s):
+    if own:
+        return _run_own(s)
+    if s["op"] == "embed":
+        return _plain_embed(s)
+    if s["op"] == "dropout":
+        m = _plain_factor(s)
+        return {"y": (s["x"].float() * m).to(s["x"].dtype), "dx": (s["dy"].float() * m).to(s["x"].dtype)}
+    return _plain_norm(s)
+
+
+def _run_own(s):
+    ops = _ops()
+    if s["op"] == "embed":
+        out = {"y": ops.embedding_forward(s["ids"], s["table"], scale=s["scale"])}
+        if s["train"]:
+            out["dtable"] = ops.embedding_backward(s["dy"], s["ids"], s["V"], scale=s["scale"])
+        return out
+    if s["op"] == "dropout":
+        return {"y": ops.dropout_apply(s["x"], s["p"], s["seed"], step=s["step"]),
+                "dx": ops.dropout_apply(s["dy"], s["p"], s["seed"], step=s["step"])}
+    y, mean, rstd = ops.layer_norm_forward(s["x"], s["w"], s["b"], eps=_EPS, p=s["p"], seed=s["seed"], step=s["step"],
+                                           stats=s["train"])
+    if not s["train"]:
+        return {"y": y}
+    dx, dw, db = ops.layer_norm_backward(s["dy"], s["x"], mean, rstd, s["w"], s["b"], p=s["p"], seed=s["seed"],
+                                         step=s["step"])
+    return {"y": y, "mean": mean, "rstd": rstd, "dx": dx, "dw": dw, "db": db}
+
+
+def _plain_norm(s):
+    x = s["x"].float()
+    mean = x.mean(dim=1, keepdim=True)
+    xc = x - mean
+    rstd = torch.rsqrt((xc * xc).mean(dim=1, keepdim=True) + _EPS)
+    xh = xc * rstd
+    u = xh * s["w"] + s["b"]
+    m = _plain_factor(s) if s["p"] > 0 else None
+    y = (u if m is None else u * m).to(s["x"].dtype)
+    if not s["train"]:
+        return {"y": y}
+    du = s["dy"].float() if m is None else s["dy"].float() * m
+    db = du.sum(dim=0)
+    dw = (du * xh).sum(dim=0)
+    g = du * s["w"]
+    dx = rstd * (g - g.mean(dim=1, keepdim=True) - xh * (g * xh).mean(dim=1, keepdim=True))
+    return {"y": y, "mean": mean[:, 0], "rstd": rstd[:, 0], "dx": dx.to(s["x"].dtype), "dw": dw, "db": db}
+
+
+def _plain_embed(s):
+    ids, table = s["ids"], s["table"]
+    some = (ids >= 0) & (ids < s["V"])
+    rows = table[torch.where(some, ids, 0)].float() * s["scale"]
+    out = {"y": torch.where(some[:, None], rows, 0.0).to(table.dtype)}
+    if s["train"]:  # tokens sorted by row; a row's sum is a difference of running sums (in 64 bits)
+        key, order = torch.where(some, ids, s["V"]).sort(stable=True)
+        T, N = s["dy"].shape
+        blocks = torch.zeros((T + 511) // 512, 512, N, dtype=torch.float64, device="cuda")
+        blocks.view(-1, N)[:T] = s["dy"][order].double()
+        blocks = blocks.cumsum(1)
+        blocks[1:] += blocks[:-1, -1].cumsum(0)[:, None]
+        total = torch.cat((torch.zeros(1, N, dtype=torch.float64, device="cuda"), blocks.view(-1, N)))
+        edge = torch.searchsorted(key, torch.arange(s["V"] + 1, device="cuda"))
+        out["dtable"] = ((total[edge[1:]] - total[edge[:-1]]) * s["scale"]).to(table.dtype)
+    return out
+
+
+def _plain_factor(s):
+    """The dropout factor [M, N] in 32 bits: 0 or 1 / P(kept)."""
+    M, N = s["M"], s["N"]
+    low = 0xFFFFFFFF
+    groups = (N + 7) // 8
+    c0 = torch.arange(groups, device="cuda").expand(M, groups)
+    c1 = torch.arange(M, device="cuda")[:, None].expand(M, groups)
+    c2 = torch.full((M, groups), s["step"] & low, device="cuda", dtype=torch.int64)
+    c3 = torch.full((M, groups), (s["step"] >> 32) & low, device="cuda", dtype=torch.int64)
+    k0, k1 = s["seed"] & low, (s["seed"] >> 32) & low
+    for _ in range(10):  # (the product's 64 bits, in two's complement)
+        p0, p1 = c0 * 0xD2511F53, c2 * 0xCD9E8D57
+        c0, c1, c2, c3 = ((p1 >> 32) & low) ^ c1 ^ k0, p1 & low, ((p0 >> 32) & low) ^ c3 ^ k1, p0 & low
+        k0, k1 = (k0 + 0x9E3779B9) & low, (k1 + 0xBB67AE85) & low
+    half = torch.stack((c0 & 0xFFFF, c0 >> 16, c1 & 0xFFFF, c1 >> 16, c2 & 0xFFFF, c2 >> 16, c3 & 0xFFFF, c3 >> 16), dim=2)
+    thr = int(math.floor(s["p"] * 65536 + 0.5))
+    kept = half.reshape(M, groups * 8)[:, :N] >= thr
+    return torch.where(kept, 65536.0 / (65536 - thr) if thr < 65536 else 0.0, 0.0)
+
+
+# ---- what a pass cannot do without -----------------------------------------------------------
+def work(case):
+    z = _SIZE[case["type"]]
+    if case["op"] == "embed":
+        t, v, n = case["T"], case["V"], case["N"]
+        size = 8 * t + min(t, v) * n * z + t * n * z
+        flops = t * n
+        if case["train"]:
+            size += t * n * z + v * n * z
+            flops += 2 * t * n
+        return {"bytes": size, "flops": flops}
+    e = case["M"] * case["N"]
+    if case["op"] == "dropout":
+        return {"bytes": 4 * e * z, "flops": 2 * e}
+    if not case["train"]:
+        return {"bytes": 2 * e * z + 8 * case["N"], "flops": 8 * e}
+    return {"bytes": 4 * e * z + 16 * case["N"] + 8 * case["M"], "flops": 22 * e}
+
+
+# ---- the definitions in 64 bits --------------------------------------------------------------
+def _exact_factor(case, s):
+    """The dropout factor in 64 bits, the generator on the host in unsigned 64-bit words."""
+    M, N = case["M"], case["N"]
+    word = np.uint64
+    g = (N + 7) // 8
+    mask = word(0xFFFFFFFF)
+    ctr = [np.tile(np.arange(g, dtype=word), M), np.repeat(np.arange(M, dtype=word), g),
+           np.full(M * g, s["step"] % 2**32, dtype=word), np.full(M * g, s["step"] // 2**32, dtype=word)]
+    key = [s["seed"] % 2**32, s["seed"] // 2**32]
+    for _ in range(10):
+        a, b = ctr[0] * word(0xD2511F53), ctr[2] * word(0xCD9E8D57)
+        ctr = [(b >> word(32)) ^ ctr[1] ^ word(key[0]), b & mask, (a >> word(32)) ^ ctr[3] ^ word(key[1]), a & mask]
+        key = [(key[0] + 0x9E3779B9) % 2**32, (key[1] + 0xBB67AE85) % 2**32]
+    words = np.stack(ctr, axis=1).astype("<u4")
+    bits = words.view("<u2").reshape(M, g * 8)[:, :N]
+    thr = int(case["p"] * 65536 + 0.5)
+    keep = torch.from_numpy((bits >= thr)).cuda()
+    return keep.double() * (65536 / (65536 - thr) if thr < 65536 else 0.0)
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    if case["op"] == "embed":
+        ids, table = s["ids"], s["table"].double()
+        none = (ids < 0) | (ids >= case["V"])
+        y = table.index_select(0, ids.masked_fill(none, 0)) * s["scale"]
+        y[none] = 0
+        out = {"y": y}
+        if case["train"]:
+            total = torch.zeros(case["V"] + 1, case["N"], dtype=torch.float64, device="cuda")
+            total.index_add_(0, ids.masked_fill(none, case["V"]), s["dy"].double())
+            out["dtable"] = total[:-1] * s["scale"]
+        return out
+    if case["op"] == "dropout":
+        f = _exact_factor(case, s)
+        return {"y": s["x"].double() * f, "dx": s["dy"].double() * f}
+    x = s["x"].double()
+    n = case["N"]
+    mean = x.sum(1) / n
+    var = torch.var(x, dim=1, unbiased=False)
+    rstd = (var + _EPS) ** -0.5
+    xh = (x - mean[:, None]) * rstd[:, None]
+    w = s["w"].double()
+    f = _exact_factor(case, s) if case["p"] > 0 else 1.0
+    out = {"y": torch.addcmul(s["b"].double(), xh, w) * f}
+    if case["train"]:
+        du = s["dy"].double() * f
+        a = du * w
+        c1, c2 = a.sum(1) / n, torch.linalg.vecdot(a, xh, dim=1) / n
+        out |= {"mean": mean, "rstd": rstd, "dw": torch.linalg.vecdot(du, xh, dim=0), "db": du.sum(0),
+                "dx": (a - torch.outer(c1, torch.ones_like(w)) - xh * c2[:, None]) * rstd[:, None]}
+    return out
