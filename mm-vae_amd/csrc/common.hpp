@@ -299,14 +299,10 @@ MMVAE_DEV float softplus_sig(float u, float& sig) {
 MMVAE_DEV float clamp_nu(float sp) { return __builtin_amdgcn_fmed3f(sp, 1e-4f, 1e4f); }
 
 // ---------------------------------------------------------------------------------------
-// Packed f32 pairs (v_pk_fma_f32 / v_pk_mul_f32 / v_pk_add_f32): one issue covers two
-// elements, which halves the issue cost of a VALU-issue-bound loop run by one wave per SIMD.
+// Row pairs: two elements as two scalar f32 streams.  The packed f32 instructions are off for all
+// device code (Makefile: some of their forms have given wrong results now and then); the NB step
+// takes 0.524 ms without them, 0.519 ms with them (1M x 20k, B = 4096, bf16x3).
 // ---------------------------------------------------------------------------------------
-#ifndef MMVAE_F2_SCALAR
-typedef float f2 __attribute__((ext_vector_type(2)));
-MMVAE_DEV f2 fma2(f2 a, f2 b, f2 c) { return __builtin_elementwise_fma(a, b, c); }
-#else
-// the same row-pair code as two scalar f32 streams (v_fma_f32 / v_mul_f32 / v_add_f32)
 struct f2 {
     float x, y;
     MMVAE_DEV float& operator[](int i) { return i ? y : x; }
@@ -326,7 +322,6 @@ MMVAE_DEV f2 operator-(float a, f2 b) { return f2{a - b.x, a - b.y}; }
 MMVAE_DEV f2 operator*(float a, f2 b) { return f2{a * b.x, a * b.y}; }
 MMVAE_DEV f2 operator-(f2 a) { return f2{-a.x, -a.y}; }
 MMVAE_DEV f2 fma2(f2 a, f2 b, f2 c) { return f2{fmaf(a.x, b.x, c.x), fmaf(a.y, b.y, c.y)}; }
-#endif
 MMVAE_DEV f2 splat2(float v) { return f2{v, v}; }
 
 // Dense NB terms of two (cell, gene) elements at x = 0 (nb.hh:456-459, 518-528) — nb_nu2 is its
@@ -433,22 +428,13 @@ MMVAE_DEV void nb_gamma_terms(float nup, float x, float& lgd, float& dgd, const 
     }
 }
 
-// nb_gamma_terms of two counts that are integers in 0..8 (0: lgd = dgd = 0), as packed pairs.
-// Factor i of the finite product is nup + i while i < x, else 1 — on_i = clamp(x - i, 0, 1) is one
-// v_pk_add_f32 with the clamp modifier, a_i = on_i (nup + i) + (1 - on_i) — so both counts of a
-// pair share every instruction instead of one select chain per count.  x0 / x1: the counts as ints.
-#ifndef MMVAE_F2_SCALAR
-MMVAE_DEV f2 clamp01_add2(f2 x, float c) {  // min(max(x + c, 0), 1) per half, c wave-uniform
-    f2 o;  // (a 64-bit SGPR pair operand whose low word, c, feeds both halves: op_sel_hi)
-    const uint64_t cp = (uint64_t)__float_as_uint(c);
-    asm("v_pk_add_f32 %0, %1, %2 op_sel_hi:[1,0] clamp" : "=v"(o) : "v"(x), "s"(cp));
-    return o;
-}
-#else
-MMVAE_DEV f2 clamp01_add2(f2 x, float c) {
+// nb_gamma_terms of two counts that are integers in 0..8 (0: lgd = dgd = 0), as a pair.
+// Factor i of the finite product is nup + i while i < x, else 1: on_i = clamp(x - i, 0, 1),
+// a_i = on_i (nup + i) + (1 - on_i), so both counts share the instruction stream instead of one
+// select chain per count.  x0 / x1: the counts as ints.
+MMVAE_DEV f2 clamp01_add2(f2 x, float c) {  // min(max(x + c, 0), 1) of each
     return f2{fminf(fmaxf(x.x + c, 0.f), 1.f), fminf(fmaxf(x.y + c, 0.f), 1.f)};
 }
-#endif
 MMVAE_DEV void nb_gamma_terms2(f2 nup, f2 x, int x0, int x1, f2& lgd, f2& dgd, const float* ftab) {
     constexpr float LN2 = 0.6931471805599453f;
     f2 P = splat2(1.f), Pd = splat2(0.f);

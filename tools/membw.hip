@@ -1,6 +1,6 @@
 // Write / read bandwidth of the access shapes the wide path's [B, D] blocks see (a probe, not part
 // of the engine): whole rows, MFMA-layout tiles (16 lanes x 4 B per row, 4 rows an instruction)
-// and float4 tiles, over a 4096 x 20000 f32 block.   hipcc -O3 --offload-arch=gfx950 membw.hip
+// and float4 tiles, over a 4096 x 20000 f32 block.   hipcc -O3 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops membw.hip
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

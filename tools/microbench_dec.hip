@@ -1,5 +1,5 @@
 // Micro-benchmark of the decoder pass-A inner loop with ablations (diagnostic tool, not shipped).
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 tools/microbench_dec.hip -o /tmp/mb && /tmp/mb
+//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops tools/microbench_dec.hip -o /tmp/mb && /tmp/mb
 // Variant bits: 1 = skip W loads (reuse registers), 2 = skip MFMA, 4 = skip epilogue.
 #include <hip/hip_runtime.h>
 #include <cstdio>
