@@ -246,6 +246,106 @@ int mmvae_debug_poison(mmvae_h h, int32_t byte);
 int mmvae_graph_enable(mmvae_h h, int32_t on);
 int mmvae_graph_stats(mmvae_h h, int64_t* captures, int64_t* replays);
 
+/* ---- layer operators on device tensors ------------------------------------------------
+ * Layer norm (with an optional ReLU and dropout in the same pass), dropout and embedding lookup,
+ * forward and backward, on row-major device arrays of the caller: the hidden-layer chain of the
+ * wide path, callable on its own.  No handle: `device` is the HIP device of every pointer,
+ * `stream` a hipStream_t of it (NULL: its default stream); the calling thread's current device is
+ * the same after the call.  The calls only enqueue kernels (no allocation, synchronisation,
+ * memset or copy), so they can be captured into a HIP graph; a captured call's buffers, the
+ * workspace among them, belong to that graph.  Different threads may call at the same time.
+ * Errors: MMVAE_E_ARG before anything is enqueued, MMVAE_E_HIP; message by mmvae_last_error(NULL).
+ * Row strides (ld*) count elements; inputs may repeat rows (stride 0), outputs may not overlap.
+ * Every sum is f32 in a fixed order (equal calls give equal bits); results are rounded to their
+ * type once, to nearest even. */
+enum { MMVAE_T_F32 = 0, MMVAE_T_BF16 = 1, MMVAE_T_F16 = 2 };
+
+/* Dropout with probability p in [0, 1]: 16 random bits per element, half (col % 8) of the words
+ * of Philox4x32-10 under the key (seed, seed >> 32) at the counter (col / 8, row, step,
+ * step >> 32 ^ row >> 32), row = row_offset + r; the element is kept, times 65536 / (65536 - thr),
+ * iff they are >= thr = floor(65536 p + 1/2).  A function of (seed, step, row, col) alone, like the
+ * reparameterisation noise: shards of a batch drop what the whole batch would, a backward call
+ * with the forward's key recomputes its mask.  `state` (device int64[2] or NULL) is added to
+ * (step, row_offset) by the kernel: a captured graph's replays read new values from it. */
+
+/* y = drop(act(xh w + b)), xh = (x - mean(x)) / sqrt(var(x) + eps) over each row of N;
+ * act: ReLU if relu != 0 (its gradient at 0 is 0).
+ * Backward (du = dy times the dropout factor and ReLU mask, g = du w):
+ *   dx = rstd (g - mean(g) - xh mean(g xh)), dw = sum_rows du xh, db = sum_rows du.
+ * y may be x, and dx may be dy or x, at the same row stride. */
+typedef struct mmvae_norm_args {
+    int64_t M, N;              /* rows, columns: 0 <= M, 1 <= N, both < 2^31 - 65536 */
+    const void *x;
+    int64_t ldx;
+    const void *w, *b;         /* [N] of type wtype; NULL: 1 and 0 */
+    void *y;                   /* forward */
+    int64_t ldy;
+    float *mean, *rstd;        /* [M]: forward, written (NULL: not); backward, read */
+    const void *dy;            /* backward */
+    int64_t lddy;
+    void *dx;                  /* NULL: not computed */
+    int64_t lddx;
+    void *dw, *db;             /* [N] of type wtype; NULL: not computed */
+    void *ws;                  /* backward with dw or db: mmvae_layer_norm_bwd_ws(M, N) bytes */
+    int64_t ws_bytes;
+    double p;                  /* dropout probability, 0: none */
+    uint64_t seed, step, row_offset;
+    const int64_t *state;
+    void *stream;
+    int32_t device;
+    int32_t dtype, wtype;      /* MMVAE_T_*: x, y, dy, dx; w, b, dw, db (dtype or F32) */
+    float eps;
+    int32_t relu;
+    int32_t reserved;
+} mmvae_norm_args;
+int mmvae_layer_norm_fwd(const mmvae_norm_args* args);
+int mmvae_layer_norm_bwd(const mmvae_norm_args* args);
+int64_t mmvae_layer_norm_bwd_ws(int64_t M, int64_t N);
+
+/* y[r][c] = x[r][c] times its dropout factor; a dropped element is 0 whatever x holds.  The
+ * gradient is the same call on dy.  y may be x. */
+typedef struct mmvae_dropout_args {
+    int64_t M, N;
+    const void *x;
+    int64_t ldx;
+    void *y;
+    int64_t ldy;
+    double p;
+    uint64_t seed, step, row_offset;
+    const int64_t *state;
+    void *stream;
+    int32_t device;
+    int32_t dtype;
+} mmvae_dropout_args;
+int mmvae_dropout(const mmvae_dropout_args* args);
+
+/* y[t] = scale table[ids[t]] (+ add[t]); an id outside [0, V) (a cell without a label) looks up
+ * zeros and has no gradient.  Backward: dtable[v] = scale sum of dy[t] over ids[t] = v, every row
+ * of [V][N] written (contiguous, 4-byte aligned), the tokens summed in a fixed order. */
+typedef struct mmvae_embedding_args {
+    int64_t T, N, V;           /* tokens, width (< 2^24), table rows; T, V < 2^31 - 65536 */
+    const void *ids;           /* [T] int64 (ids64 != 0) or int32 */
+    const void *table;         /* forward */
+    int64_t ldt;
+    const void *add;           /* [T][N] or NULL */
+    int64_t ldadd;
+    void *y;
+    int64_t ldy;
+    const void *dy;            /* backward */
+    int64_t lddy;
+    void *dtable;
+    void *ws;                  /* backward: mmvae_embedding_bwd_ws(T, N) bytes */
+    int64_t ws_bytes;
+    void *stream;
+    int32_t device;
+    int32_t dtype;             /* MMVAE_T_*: table, add, y, dy, dtable */
+    int32_t ids64;
+    float scale;
+} mmvae_embedding_args;
+int mmvae_embedding_fwd(const mmvae_embedding_args* args);
+int mmvae_embedding_bwd(const mmvae_embedding_args* args);
+int64_t mmvae_embedding_bwd_ws(int64_t T, int64_t N);
+
 /* ---- operators.hh (vMF observation model scalars) ----------------------------------
  * lbessel(kappa, nu): piecewise log I_nu(kappa) approximation (operators.hh:49-101) with
  * P. Mineiro's fasterlgamma (fastgamma.h:58-60); its custom backward returns the Baricz

@@ -15,6 +15,7 @@
 #include "../../include/mmvae/lbessel.hh"
 #include "common.hpp"
 #include "engine.hpp"
+#include "ops.hpp"
 #include "tiles.hpp"
 
 using namespace mmvae;
@@ -37,6 +38,14 @@ static thread_local std::string g_last_error;
     } while (0)
 
 namespace mmvae {
+
+int set_last_error(int code, const char* op, const char* msg) noexcept {
+    try {
+        g_last_error = std::string(op) + ": " + msg;
+    } catch (...) {  // (no memory for the message: the code still says what happened)
+    }
+    return code;
+}
 
 void timer_begin(Engine* e, const char* name, hipEvent_t* a) {
     auto it = e->timer_index.find(name);

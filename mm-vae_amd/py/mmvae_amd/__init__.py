@@ -101,6 +101,14 @@ def lib():
         "mmvae_lbessel_grad": (ctypes.c_float, [ctypes.c_float, ctypes.c_float]),
         "mmvae_fasterlog": (ctypes.c_float, [ctypes.c_float]),
         "mmvae_fasterlgamma": (ctypes.c_float, [ctypes.c_float]),
+        # (the layer operators' argument structs travel packed: ops.py)
+        "mmvae_layer_norm_fwd": (ctypes.c_int, [ctypes.c_char_p]),
+        "mmvae_layer_norm_bwd": (ctypes.c_int, [ctypes.c_char_p]),
+        "mmvae_layer_norm_bwd_ws": (i64, [i64, i64]),
+        "mmvae_dropout": (ctypes.c_int, [ctypes.c_char_p]),
+        "mmvae_embedding_fwd": (ctypes.c_int, [ctypes.c_char_p]),
+        "mmvae_embedding_bwd": (ctypes.c_int, [ctypes.c_char_p]),
+        "mmvae_embedding_bwd_ws": (i64, [i64, i64]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)

@@ -1,0 +1,101 @@
+"""Test infrastructure: the layer operators (mmvae_amd.ops) in 64 bits on the CPU, from their formulas.
+
+The reference has no such layers; these are the definitions the operators' documentation states, with
+the error bounds that 32-bit evaluation of them has."""
+import numpy as np
+import torch
+
+from . import philox
+
+U32 = 2.0 ** -24  # half a step of float32, relative
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def drop_threshold(p):
+    return int(np.floor(p * 65536 + 0.5))
+
+
+def drop_kept(M, N, p, seed, step=0, row_offset=0):
+    """The kept elements [M, N]: half col % 8 of philox(col / 8, row, step, step >> 32 ^ row >> 32) >= threshold."""
+    rows = (np.arange(M, dtype=np.uint64) + np.uint64(row_offset))[:, None]
+    grp = np.arange((N + 7) // 8, dtype=np.uint64)[None, :]
+    shape = (M, grp.shape[1])
+    seed, step = seed % 2 ** 64, step % 2 ** 64
+    c = philox._philox4x32_10(np.broadcast_to(grp, shape), np.broadcast_to(rows & np.uint64(0xFFFFFFFF), shape),
+                              np.full(shape, np.uint64(step & 0xFFFFFFFF)),
+                              np.broadcast_to((rows >> np.uint64(32)) ^ np.uint64(step >> 32), shape),
+                              seed & 0xFFFFFFFF, seed >> 32)
+    halves = np.stack([h for w in c for h in (w & np.uint64(0xFFFF), w >> np.uint64(16))], axis=2)
+    return torch.from_numpy(halves.reshape(M, -1)[:, :N] >= drop_threshold(p))
+
+
+def drop_scale(p):
+    t = drop_threshold(p)
+    return 65536 / (65536 - t) if t < 65536 else 0.0
+
+
+def drop_factor(M, N, p, seed, step=0, row_offset=0):
+    return torch.where(drop_kept(M, N, p, seed, step, row_offset), drop_scale(p), 0.0).double() if p > 0 else torch.ones(M, N).double()
+
+
+def norm(x, w, b, eps, factor, relu):
+    """y, mean, rstd, u (before ReLU and dropout) of float64 tensors."""
+    mean = x.mean(1, keepdim=True)
+    rstd = 1 / torch.sqrt(((x - mean) ** 2).mean(1, keepdim=True) + eps)
+    u = (x - mean) * rstd * w + b
+    y = (u.clamp(min=0) if relu else u) * factor
+    return y, mean[:, 0], rstd[:, 0], u
+
+
+def norm_grads(dy, x, w, eps, factor, mask):
+    """dx, dw, db and the error bounds of their 32-bit evaluation (before the final rounding), with the ReLU's mask."""
+    M, N = x.shape
+    mean = x.mean(1, keepdim=True)
+    rstd = 1 / torch.sqrt(((x - mean) ** 2).mean(1, keepdim=True) + eps)
+    xh = (x - mean) * rstd
+    du = dy * factor * mask
+    g = du * w
+    c1, c2 = g.mean(1, keepdim=True), (g * xh).mean(1, keepdim=True)
+    dx = rstd * (g - c1 - xh * c2)
+    # A row's sums are chains of at most ROW additions, so the mean is off by ROW u mean|x|, xh by
+    # ROW u A with A = rstd mean|x| + |xh| + 1, and the means of g and g xh by ROW u of their absolute sums.
+    a = rstd * x.abs().mean(1, keepdim=True) + xh.abs() + 1
+    ag = (g.abs() * a).mean(1, keepdim=True)
+    bdx = ROW * U32 * rstd * (2 * g.abs() + 2 * g.abs().mean(1, keepdim=True) + 2 * a * (g * xh).abs().mean(1, keepdim=True) + xh.abs() * 2 * ag)
+    dw, db = (du * xh).sum(0), du.sum(0)
+    # A column's sums: at most M / 256 + 96 additions (a thread's rows, the workgroup's, the partial rows')
+    col = M / 256 + 96
+    return dx, dw, db, bdx, U32 * ((col + ROW) * (du.abs() * a).sum(0)), U32 * col * du.abs().sum(0)
+
+
+# additions in a row's sum: a thread's 8 x 4 elements, 6 lane steps, 16 waves; in sweeps (N > 32768) 8 + N / 8192
+ROW = 72
+
+
+def norm_bound(x, w, b, eps, factor):
+    """The error bound of y before its final rounding: xh as above, times |w|, and the roundings of u."""
+    mean = x.mean(1, keepdim=True)
+    rstd = 1 / torch.sqrt(((x - mean) ** 2).mean(1, keepdim=True) + eps)
+    xh = (x - mean) * rstd
+    a = rstd * x.abs().mean(1, keepdim=True) + xh.abs() + 1
+    return U32 * (ROW * a * w.abs() + 2 * b.abs()) * factor
+
+
+def embedding(ids, table, scale, add=None):
+    ok = (ids >= 0) & (ids < table.shape[0])
+    y = torch.where(ok[..., None], table[torch.where(ok, ids, 0)] * scale, 0.0) if table.shape[0] else torch.zeros(*ids.shape, table.shape[1]).double()
+    return y if add is None else y + add
+
+
+def embedding_grad(dy, ids, rows, scale):
+    """The table's gradient and the bound of its 32-bit sum: chains of at most 128 additions (32 of a group,
+    32 groups, the pieces of a run and their groups), the scale's rounding."""
+    ok = (ids >= 0) & (ids < rows)
+    i = torch.where(ok, ids, rows).reshape(-1).long()
+    d = dy.reshape(-1, dy.shape[-1])
+    out = torch.zeros(rows + 1, d.shape[1]).double().index_add_(0, i, d)
+    mag = torch.zeros(rows + 1, d.shape[1]).double().index_add_(0, i, d.abs())
+    return out[:rows] * scale, 130 * U32 * abs(scale) * mag[:rows]

@@ -1,0 +1,189 @@
+"""CPU tests of the layer operators' boundary (include/mmvae_capi.h, mmvae_amd.ops): the packed argument
+structs match the header's, every wrong call is refused before a device is touched, the oracle's own
+formulas hold against differences, and the dropout masks have the stated rate."""
+import ctypes
+import os
+import re
+import subprocess
+
+import numpy as np
+import pytest
+import torch
+
+import mmvae_amd
+from mmvae_amd import ops
+from oracle import layers
+
+INCLUDE = os.path.dirname(mmvae_amd.HEADER_PATH)
+
+
+def pack_norm(**kw):
+    v = dict(M=4, N=8, x=4096, ldx=8, w=0, b=0, y=4096, ldy=8, mean=4096, rstd=4096, dy=4096, lddy=8, dx=4096, lddx=8, dw=4096, db=4096,
+             ws=4096, ws_bytes=1 << 30, p=0.0, seed=1, step=0, row_offset=0, state=0, stream=0, device=0, dtype=0, wtype=0, eps=1e-5, relu=0, reserved=0)
+    v.update(kw)
+    return ops._NORM.pack(*v.values())
+
+
+def pack_drop(**kw):
+    v = dict(M=4, N=8, x=4096, ldx=8, y=4096, ldy=8, p=0.5, seed=1, step=0, row_offset=0, state=0, stream=0, device=0, dtype=0)
+    v.update(kw)
+    return ops._DROP.pack(*v.values())
+
+
+def pack_emb(**kw):
+    v = dict(T=4, N=8, V=3, ids=4096, table=4096, ldt=8, add=0, ldadd=8, y=4096, ldy=8, dy=4096, lddy=8, dtable=4096, ws=4096,
+             ws_bytes=1 << 30, stream=0, device=0, dtype=0, ids64=1, scale=1.0)
+    v.update(kw)
+    return ops._EMB.pack(*v.values())
+
+
+def test_packed_structs_match_the_header(tmp_path):
+    """Every member of the C structs lies where struct.pack puts it: distinct values written in Python, read in C."""
+    src = open(mmvae_amd.HEADER_PATH).read()
+    lines = []
+    for name in ("norm", "dropout", "embedding"):
+        body = re.sub(r"/\*.*?\*/", "", re.search(r"typedef struct mmvae_%s_args \{(.*?)\} mmvae_%s_args;" % (name, name), src, re.S).group(1), flags=re.S)
+        lines.append('printf("%s %%zu", sizeof(mmvae_%s_args));' % (name, name))
+        for decl in body.split(";"):
+            for member in decl.split(","):
+                if member.strip():
+                    m = member.split()[-1].strip("*")
+                    lines.append('printf(" %%zu", offsetof(mmvae_%s_args, %s));' % (name, m))
+        lines.append('printf("\\n");')
+    c = tmp_path / "o.c"
+    c.write_text("#include <stddef.h>\n#include <stdio.h>\n#include \"mmvae_capi.h\"\nint main(void) {%s return 0; }\n" % "\n".join(lines))
+    subprocess.run(["gcc", "-I", INCLUDE, str(c), "-o", str(tmp_path / "o")], check=True)
+    out = subprocess.run([str(tmp_path / "o")], check=True, capture_output=True, text=True).stdout.splitlines()
+    for line, st in zip(out, (ops._NORM, ops._DROP, ops._EMB)):
+        size, *offs = [int(v) for v in line.split()[1:]]
+        assert size >= st.size and size - st.size < 8, line
+        want, at = [], 0
+        for n, code in re.findall(r"(\d*)([a-zA-Z])", st.format[1:]):
+            for _ in range(int(n or 1)):
+                want.append(at)
+                at += {"q": 8, "Q": 8, "d": 8, "i": 4, "f": 4}[code]
+        assert offs == want, line
+
+
+NORM_BAD = [dict(M=-1), dict(N=0), dict(M=2 ** 31), dict(N=2 ** 31), dict(dtype=3), dict(wtype=1), dict(dtype=1, wtype=2), dict(eps=-1e-6),
+            dict(eps=float("nan")), dict(eps=float("inf")), dict(p=-0.1), dict(p=1.1), dict(p=float("nan")), dict(x=0), dict(ldx=-1)]
+
+
+@pytest.mark.parametrize("kw", NORM_BAD + [dict(y=0), dict(ldy=7)])
+def test_norm_forward_refuses(kw):
+    L = mmvae_amd.lib()
+    assert L.mmvae_layer_norm_fwd(pack_norm(**kw)) == -1
+    assert L.mmvae_last_error(None).startswith(b"layer_norm_fwd: ")
+
+
+@pytest.mark.parametrize("kw", NORM_BAD + [dict(dy=0), dict(mean=0), dict(rstd=0), dict(lddx=7), dict(ws=0), dict(ws_bytes=8), dict(lddy=-8)])
+def test_norm_backward_refuses(kw):
+    assert mmvae_amd.lib().mmvae_layer_norm_bwd(pack_norm(**kw)) == -1
+
+
+@pytest.mark.parametrize("kw", [dict(M=-1), dict(N=-1), dict(N=2 ** 31), dict(dtype=5), dict(p=-1.0), dict(p=2.0), dict(p=float("nan")), dict(x=0),
+                                dict(y=0), dict(ldx=-8), dict(ldy=7)])
+def test_dropout_refuses(kw):
+    assert mmvae_amd.lib().mmvae_dropout(pack_drop(**kw)) == -1
+
+
+@pytest.mark.parametrize("kw", [dict(T=-1), dict(N=0), dict(N=1 << 24), dict(V=-1), dict(V=2 ** 31), dict(T=2 ** 31), dict(dtype=-1), dict(ids=0),
+                                dict(table=0), dict(y=0), dict(ldt=-1), dict(ldadd=-1), dict(ldy=7)])
+def test_embedding_forward_refuses(kw):
+    assert mmvae_amd.lib().mmvae_embedding_fwd(pack_emb(**kw)) == -1
+
+
+@pytest.mark.parametrize("kw", [dict(T=-1), dict(N=0), dict(V=-1), dict(dtype=3), dict(ids=0), dict(dy=0), dict(dtable=0), dict(dtable=4098), dict(lddy=-1),
+                                dict(ws=0), dict(ws_bytes=100)])
+def test_embedding_backward_refuses(kw):
+    assert mmvae_amd.lib().mmvae_embedding_bwd(pack_emb(**kw)) == -1
+
+
+def test_null_arguments_refused():
+    L = mmvae_amd.lib()
+    for f in ("mmvae_layer_norm_fwd", "mmvae_layer_norm_bwd", "mmvae_dropout", "mmvae_embedding_fwd", "mmvae_embedding_bwd"):
+        assert getattr(L, f)(None) == -1
+
+
+def test_workspace_sizes_grow_with_the_call():
+    L = mmvae_amd.lib()
+    assert L.mmvae_layer_norm_bwd_ws(-1, 8) == 0 and L.mmvae_layer_norm_bwd_ws(4, 0) == 0
+    assert L.mmvae_embedding_bwd_ws(-1, 8) == 0 and L.mmvae_embedding_bwd_ws(4, 0) == 0
+    for N in (1, 7, 64, 100, 1000, 20000, 32768, 32769, 100000):
+        for M in (0, 1, 2, 100, 4096):
+            assert L.mmvae_layer_norm_bwd_ws(M, N) >= 2 * 4 * N
+    # two sorted copies of the tokens (id, position), and a partial head and tail of a piece at least
+    for T in (1, 4096, 4097, 600000):
+        assert L.mmvae_embedding_bwd_ws(T, 33) >= 16 * T + 2 * 4 * 40
+
+
+@pytest.mark.parametrize("call", [
+    lambda t: ops.layer_norm(t),
+    lambda t: ops.layer_norm_backward(t, t, t, t),
+    lambda t: ops.dropout(t, 0.5, 1),
+    lambda t: ops.embedding(torch.zeros(2, dtype=torch.int64), t),
+    lambda t: ops.embedding_backward(t, torch.zeros(2, dtype=torch.int64), 3),
+])
+def test_cpu_tensors_refused(call):
+    with pytest.raises(mmvae_amd.MMVAEError, match="CUDA"):
+        call(torch.zeros(2, 4))
+
+
+@pytest.mark.parametrize("relu", [False, True])
+def test_oracle_gradients_against_differences(relu):
+    """The formulas' gradients against central differences of the 64-bit forward (h = 1e-6: truncation and
+    rounding both below 1e-8 of values of order 1)."""
+    rng = np.random.default_rng(5)
+    M, N, eps, p, seed = 5, 11, 1e-5, 0.3, 77
+    x, dy = (torch.from_numpy(rng.normal(size=(M, N))) for _ in range(2))
+    w, b = torch.from_numpy(1 + 0.2 * rng.normal(size=N)), torch.from_numpy(0.2 * rng.normal(size=N))
+    f = layers.drop_factor(M, N, p, seed)
+    u = layers.norm(x, w, b, eps, f, relu)[3]
+    mask = (u > 0).double() if relu else torch.ones_like(u)
+    assert u.abs().min() > 1e-3  # (no element near the ReLU's corner for the differences)
+    dx, dw, db = layers.norm_grads(dy, x, w, eps, f, mask)[:3]
+
+    def loss(x, w, b):
+        return float((layers.norm(x, w, b, eps, f, relu)[0] * dy).sum())
+    h = 1e-6
+    for t, g, k in ((x, dx, 0), (w, dw, 1), (b, db, 2)):
+        for i in np.ndindex(*t.shape):
+            a = [x, w, b]
+            lo, hi = t.clone(), t.clone()
+            lo[i] -= h
+            hi[i] += h
+            a[k] = hi
+            up = loss(*a)
+            a[k] = lo
+            assert abs((up - loss(*a)) / (2 * h) - float(g[i])) < 1e-7
+
+
+def test_oracle_embedding_gradient_against_differences():
+    rng = np.random.default_rng(6)
+    ids = torch.tensor([2, 0, 2, -1, 5, 1, 2])  # 5: outside the table's 5 rows
+    table, dy = torch.from_numpy(rng.normal(size=(5, 3))), torch.from_numpy(rng.normal(size=(7, 3)))
+    g, _ = layers.embedding_grad(dy, ids, 5, 1.7)
+    h = 1e-6
+    for i in np.ndindex(5, 3):
+        hi, lo = table.clone(), table.clone()
+        hi[i] += h
+        lo[i] -= h
+        d = float(((layers.embedding(ids, hi, 1.7) - layers.embedding(ids, lo, 1.7)) * dy).sum()) / (2 * h)
+        assert abs(d - float(g[i])) < 1e-8
+
+
+@pytest.mark.parametrize("p", [0.0, 1e-6, 0.1, 0.5, 0.9, 1.0])
+def test_dropout_rate_and_independence(p):
+    """The kept share is 1 - thr / 65536 within 5 standard deviations; other seeds, steps and rows draw other masks."""
+    M, N = 200, 1000
+    k = layers.drop_kept(M, N, p, 123, 4)
+    q = 1 - layers.drop_threshold(p) / 65536
+    assert abs(float(k.double().mean()) - q) <= 5 * np.sqrt(q * (1 - q) / (M * N)) + 1e-12
+    assert abs(q * layers.drop_scale(p) - (1 if q > 0 else 0)) < 1e-12  # the mean is kept
+    if 0.05 < p < 0.95:
+        for other in (layers.drop_kept(M, N, p, 124, 4), layers.drop_kept(M, N, p, 123, 5), layers.drop_kept(M, N, p, 123 + 2 ** 32, 4),
+                      layers.drop_kept(M, N, p, 123, 4 + 2 ** 32)):
+            agree = float((k == other).double().mean())
+            assert abs(agree - (q * q + (1 - q) ** 2)) < 0.02
+    # a shard's rows are the whole batch's
+    assert torch.equal(layers.drop_kept(50, N, p, 123, 4, row_offset=100), k[100:150])
