@@ -76,6 +76,23 @@ typedef struct mmvae_cfg {
     int32_t n_dec_hidden;    /* NB --mean_decoding / vMF --decoding */
     int32_t enc_hidden[MMVAE_MAX_HIDDEN];
     int32_t dec_hidden[MMVAE_MAX_HIDDEN];
+    /* Regularised, label-conditioned layer chains (not in the reference; any of them: the wide path).
+     * Every Linear / Angular of the encoder chain and every hidden Linear of the decoder chain
+     * computes drop(relu?(norm(W h + b))):
+     *   layer_norm != 0: layer norm over the layer's width (eps 1e-5) with a weight and bias that
+     *     are registered (clip, Adam): "mu_enc.norm_<l>.weight|bias", "mu_dec.norm_<l>..." (NB),
+     *     "z_enc.norm_<l>...", "z_dec.norm_<l>..." (vMF), l = 1, 2, ..;
+     *   dropout, in [0, 1): the probability in the training-mode passes (update steps and the
+     *     reference's eval pass, which runs in train mode); mmvae_encode drops nothing.  The masks
+     *     are keyed by (seed, layer, step_id, global row), so data-parallel shards draw the whole
+     *     batch's, and an eval pass with a step's step_id draws that step's.
+     * n_labels > 0: the decoder reads z + label_scale E[label], E = "label_embedding.weight"
+     * [n_labels][K], registered; the cells' labels are set with mmvae_set_labels. */
+    int32_t layer_norm;
+    float dropout;
+    int64_t n_labels;
+    float label_scale;   /* default 1 */
+    int32_t reserved;
 } mmvae_cfg;
 
 /* Fill a cfg with the reference defaults (mmvae_alg.hh:19-23, nb.hh:58-61, vmf.hh:59-63). */
@@ -125,6 +142,9 @@ int mmvae_upload_csr(mmvae_h h, const int64_t* rowptr, const int32_t* col, const
  * instead of O(N nnz). */
 int mmvae_stream_csr(mmvae_h h, const int64_t* rowptr, const int32_t* col, const float* val,
                      int64_t N, int64_t D, const float* covar);
+/* The dataset cells' labels (cfg.n_labels > 0), host int32 [N]: [0, n_labels), or -1 for a cell
+ * without one.  After every upload / stream / synth call, which forget them; copied. */
+int mmvae_set_labels(mmvae_h h, const int32_t* labels, int64_t N);
 /* Dataset size after upload/synth (mtx_data_block_t::ntot / nfeature, mmvae_io.hh:73-74). */
 int mmvae_dataset_size(mmvae_h h, int64_t* N, int64_t* D);
 /* Device-side synthetic dataset (bench / smoke): SURVEY §8(d) count distribution. */

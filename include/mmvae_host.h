@@ -49,6 +49,10 @@ void mmvae_free(void* p);
 /* The all-ones covariate file the CLIs write when --covar is absent
  * (create_ones_like, mmvae_io.hh:292-310): a 1 x N gzip MatrixMarket. */
 int mmvae_mtx_write_ones(const char* path, int64_t N);
+/* Cell labels for mmvae_set_labels (the CLIs' --labels; not in the reference): text or gzip, one
+ * label per line and cell, a whole number >= 0, or -1 / NA for a cell without one; N lines.
+ * *labels [N] (free with mmvae_free), *n_labels = the largest label + 1. */
+int mmvae_labels_read(const char* path, int64_t N, int32_t** labels, int64_t* n_labels);
 /* ${mtx}.index (build_mmutil_index, mmutil_index.hh:138-190): for a column-sorted BGZF
  * MatrixMarket file, the BGZF virtual offset of every column's first line as gzip text
  * "col voff" lines (0-based columns).  index_file NULL or "" -> mtx + ".index".  An existing

@@ -215,6 +215,22 @@ static void build_registry_nb(Engine* e) {
     build_frozen_chains(e, false);
 }
 
+// the layer chains' registered parameters (cfg.layer_norm, cfg.n_labels), behind the reference's
+static void build_registry_layers(Engine* e) {
+    const bool vmf = e->cfg.model == MMVAE_MODEL_VMF;
+    if (e->cfg.layer_norm) {
+        auto norm = [&](const char* seq, int l, int64_t width) {
+            const std::string n = std::string(vmf ? "z_" : "mu_") + seq + ".norm_" + std::to_string(l + 1);
+            add_slot(e, n + ".weight", {width}, true);
+            add_slot(e, n + ".bias", {width}, true);
+        };
+        if (e->cfg.n_enc_hidden == 0) norm("enc", 0, e->K);
+        for (int l = 0; l < e->cfg.n_enc_hidden; ++l) norm("enc", l, e->cfg.enc_hidden[l]);
+        for (int l = 0; l < e->cfg.n_dec_hidden; ++l) norm("dec", l, e->cfg.dec_hidden[l]);
+    }
+    if (e->cfg.n_labels > 0) add_slot(e, "label_embedding.weight", {e->cfg.n_labels, e->K}, true);
+}
+
 template <class T>
 static hipError_t dalloc(T** p, int64_t n) {
     return hipMalloc(p, sizeof(T) * (size_t)(n > 0 ? n : 1));
@@ -252,6 +268,7 @@ void mmvae_cfg_default(mmvae_cfg* c, int32_t model) {
     c->kappa_min = 0.1f;
     c->kappa_max = 10.f;
     c->seed = 42;
+    c->label_scale = 1.f;
 }
 
 const char* mmvae_last_error(mmvae_h h) { return h ? h->err.c_str() : g_last_error.c_str(); }
@@ -281,9 +298,13 @@ int mmvae_create(const mmvae_cfg* cfg, int device, mmvae_h* out) {
         if (cfg->enc_hidden[l] < 1) FAIL((Engine*)nullptr, MMVAE_E_ARG, "hidden encoder widths must be >= 1");
     for (int l = 0; l < cfg->n_dec_hidden; ++l)
         if (cfg->dec_hidden[l] < 1) FAIL((Engine*)nullptr, MMVAE_E_ARG, "hidden decoder widths must be >= 1");
+    if (!(cfg->dropout >= 0.f && cfg->dropout < 1.f)) FAIL((Engine*)nullptr, MMVAE_E_ARG, "dropout must be in [0, 1)");
+    if (cfg->n_labels < 0 || cfg->n_labels > (int64_t(1) << 31) - 65536)
+        FAIL((Engine*)nullptr, MMVAE_E_ARG, "n_labels must be in [0, 2^31 - 65536]");
+    if (!std::isfinite(cfg->label_scale)) FAIL((Engine*)nullptr, MMVAE_E_ARG, "label_scale must be finite");
     // the fused tile kernels' shape envelope; anything else runs on the wide path (wide.hip)
     bool wide = cfg->K > 64 || cfg->C > CMAX || cfg->H > HMAX || cfg->R > RMAX || cfg->n_enc_hidden > 4 ||
-                cfg->n_dec_hidden > 4;
+                cfg->n_dec_hidden > 4 || cfg->layer_norm || cfg->dropout > 0.f || cfg->n_labels > 0;
     for (int l = 0; l < cfg->n_enc_hidden; ++l) wide = wide || cfg->enc_hidden[l] > 64;
     for (int l = 0; l < cfg->n_dec_hidden; ++l) wide = wide || cfg->dec_hidden[l] > 64;
     {  // the batch-list builder keeps a 16-row block's tile pointers in LDS (batch.hip)
@@ -322,6 +343,7 @@ int mmvae_create(const mmvae_cfg* cfg, int device, mmvae_h* out) {
     } else {
         build_registry_nb(e);
     }
+    build_registry_layers(e);
 
     // gene splits: one round of `per_cu` resident workgroups on each of the 256 CUs (the
     // occupancy the kernel's LDS / VGPR budget allows).  No tile kernel keeps split-long column
@@ -660,6 +682,7 @@ int mmvae_upload_csr(mmvae_h e, const int64_t* rowptr, const int32_t* col, const
     }
     e->N = N;
     e->N_host = N;
+    e->labels.clear();
     e->nnz = nnz;
     e->cell_nnz.resize((size_t)N);
     for (int64_t i = 0; i < N; ++i) e->cell_nnz[(size_t)i] = (int32_t)(rowptr[i + 1] - rowptr[i]);
@@ -903,6 +926,7 @@ int mmvae_stream_csr(mmvae_h e, const int64_t* rowptr, const int32_t* col, const
     e->hh_val = val;
     e->streamed = true;
     e->N_host = N;
+    e->labels.clear();
     e->N = e->Bpad;  // the device dataset: the batch's rows, row Bpad empty
     e->nnz = nnz;
     e->cell_nnz.resize((size_t)N);
@@ -934,6 +958,22 @@ int mmvae_stream_csr(mmvae_h e, const int64_t* rowptr, const int32_t* col, const
     return MMVAE_OK;
 }
 
+int mmvae_set_labels(mmvae_h e, const int32_t* labels, int64_t N) {
+    if (!e || !labels) FAIL(e, MMVAE_E_ARG, "set_labels: null");
+    if (e->cfg.n_labels < 1) FAIL(e, MMVAE_E_ARG, "set_labels: the model has no labels (n_labels)");
+    if (e->N_host < 1) FAIL(e, MMVAE_E_STATE, "set_labels: no dataset");
+    if (N != e->N_host) FAIL(e, MMVAE_E_ARG, "set_labels: N is not the dataset's number of cells");
+    for (int64_t i = 0; i < N; ++i)
+        if (labels[i] < -1 || labels[i] >= e->cfg.n_labels)
+            FAIL(e, MMVAE_E_ARG, "set_labels: label " + std::to_string(labels[i]) + " of cell " + std::to_string(i) + " is not -1 or in [0, n_labels)");
+    try {
+        e->labels.assign(labels, labels + N);
+    } catch (const std::bad_alloc&) {
+        return set_last_error(MMVAE_E_HIP, "set_labels", "out of host memory");
+    }
+    return MMVAE_OK;
+}
+
 int mmvae_dataset_size(mmvae_h e, int64_t* N, int64_t* D) {
     if (!e) FAIL(e, MMVAE_E_ARG, "dataset_size: null");
     if (N) *N = e->N_host;
@@ -951,6 +991,7 @@ int mmvae_synth_csr(mmvae_h e, int64_t N, double lib_size, uint64_t seed, int64_
     e->stage_bytes = e->stage_bytes_res;
     HIPCHK(e, synth_dataset(e, N, lib_size, seed, nnz_out));
     e->N_host = e->N;
+    e->labels.clear();
     return MMVAE_OK;
 }
 
@@ -1092,6 +1133,8 @@ int mmvae_init_params(mmvae_h e, uint64_t seed) {
             std::fill(v.begin(), v.end(), std::log(e->cfg.kappa_min));  // vmf.hh:323 (float log, Q4)
         } else if (s.name == "x_mean" || s.name == "mu_bias" || s.name == "nu_bias") {
             // zeros (nb.hh:312-315)
+        } else if (s.name.find(".norm_") != std::string::npos) {
+            std::fill(v.begin(), v.end(), s.name.back() == 't' ? 1.f : 0.f);  // weight 1, bias 0
         } else {
             const double bound = 1.0 / std::sqrt((double)fan_in_of(s));
             std::uniform_real_distribution<float> U((float)-bound, (float)bound);
@@ -1197,6 +1240,9 @@ static int stage_rows(Engine* e, const int64_t* cell_ids, const int64_t* ridx, i
         e->h_cells_pin[j] = c;
     }
     const int64_t Nv = e->N_host;  // the caller's cells (the padding marker: Nv)
+    // the rows' labels travel in the permutation's place (the wide path, where labels run, has none)
+    if (e->cfg.n_labels > 0)
+        for (int64_t j = 0; j < e->Bpad; ++j) e->h_perm_pin[j] = j < B && !e->labels.empty() ? e->labels[(size_t)e->h_cells_pin[j]] : -1;
     e->perm_active = balance && balance_rule(B, e->wide, (int64_t)e->cell_nnz.size() == Nv, e->no_balance);
     if (e->perm_active) {
         balance_rows(e, B);
@@ -1311,6 +1357,7 @@ int mmvae_run(mmvae_h e, const mmvae_step_args* a, float* loss_out, double* tota
     if (!e || !a || !a->cell_ids) FAIL(e, MMVAE_E_ARG, "run: null arguments");
     if (a->B < 1 || a->B > e->Bmax) FAIL(e, MMVAE_E_ARG, "run: B must be in [1, max_batch]");
     if (!e->d_rowptr) FAIL(e, MMVAE_E_STATE, "run: no dataset uploaded");
+    if (e->cfg.n_labels > 0 && e->labels.empty()) FAIL(e, MMVAE_E_STATE, "run: the cells' labels are not set (mmvae_set_labels)");
     const int64_t n_total = a->n_total > 0 ? a->n_total : a->B;
     HIPCHK(e, hipSetDevice(e->device));
     // step graphs holding RCCL calls: the batch-dependent buffers sized for every rank's worst

@@ -175,6 +175,7 @@ struct Engine {
     const StepScalars* d_ss = nullptr;
     bool perm_active = false;        // the last staged batch was reordered (noise keyed by d_perm)
     bool no_balance = false;         // MMVAE_NO_BALANCE at create (max-agreed over the ranks, comm_sync_capacity)
+    std::vector<int32_t> labels;     // host: every cell's label (cfg.n_labels > 0; empty: not set)
     std::vector<int32_t> cell_nnz;   // host copy of every cell's nonzero count (row balancing, lists)
     // per-step batch entry lists (batch.hip)
     // [ent_cap] uint2 of storage: the 32-bit entry words [0, ent_cap), and with ent_xm the float

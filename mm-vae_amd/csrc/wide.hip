@@ -26,6 +26,7 @@
 
 #include "common.hpp"
 #include "engine.hpp"
+#include "ops.hpp"
 #include "tiles.hpp"
 
 extern "C" float mmvae_fasterlgamma(float x);
@@ -725,7 +726,13 @@ struct WLayer {
     const float* b = nullptr;  // [out] or null (Angular)
     int in = 0, out = 0;
     bool relu = false;         // ReLU after this layer
-    float* act = nullptr;      // [Bpad][out] the layer's output (post-ReLU)
+    float* act = nullptr;      // [Bpad][out] the layer's output (post-ReLU, post-dropout)
+    // cfg.layer_norm: the Linear's output [Bpad][out] and its rows' statistics (the norm, the ReLU
+    // and the dropout run in one pass from there into act), and the weights' names
+    float *lin = nullptr, *mean = nullptr, *rstd = nullptr;
+    std::string norm;
+    bool drop = false;         // cfg.dropout after this layer
+    uint64_t seed = 0;         // its key
 };
 
 // a queued narrow column sum of the wide path (k_w_redsmall below)
@@ -782,6 +789,10 @@ struct WideState {
     __bf16 *pl_F = nullptr, *pl_E = nullptr;
     int kp_F = 0, kp_E = 0;
     float* colv = nullptr;  // [D] the short-K GEMM's combined column constants
+    // layer operators (ops.hip): their workspace, and the decoder's input z + label_scale E[label]
+    void* op_ws = nullptr;
+    int64_t op_ws_bytes = 0;
+    float* Zl = nullptr;
 };
 
 static hipError_t walloc(float** p, int64_t n) { return hipMalloc(p, sizeof(float) * (size_t)(n > 0 ? n : 1)); }
@@ -2237,6 +2248,14 @@ static void build_layers(Engine* e, WideState* w) {
     F.in = prev;
     F.out = (int)e->D;
     w->dec.push_back(F);
+    // norm and dropout after every layer of the encoder chain and every hidden layer of the decoder's
+    auto regular = [&](WLayer& L, const char* seq, size_t l, uint64_t key) {
+        if (e->cfg.layer_norm) L.norm = std::string(vmf ? "z_" : "mu_") + seq + ".norm_" + std::to_string(l + 1);
+        L.drop = e->cfg.dropout > 0.f;
+        L.seed = e->cfg.seed + 0x9E3779B97F4A7C15ull * key;  // apart from the latent noise's key
+    };
+    for (size_t l = 0; l < w->enc.size(); ++l) regular(w->enc[l], "enc", l, 1 + l);
+    for (size_t l = 0; l + 1 < w->dec.size(); ++l) regular(w->dec[l], "dec", l, 101 + l);
 }
 
 // frozen pointers of the layers (every frozen reload: the slots do not move, but the vMF
@@ -2312,6 +2331,22 @@ hipError_t wide_create(Engine* e) {
     WA(w->dT1, Bp * maxw);
     if (e->cfg.model == MMVAE_MODEL_VMF) WA(w->wtil, wsum);
     WA(w->lossv, 8);
+    auto norm_bufs = [&](WLayer& L) -> hipError_t {
+        if (L.norm.empty()) return hipSuccess;
+        WA(L.lin, Bp * L.out);
+        WA(L.mean, Bp);
+        WA(L.rstd, Bp);
+        w->op_ws_bytes = std::max(w->op_ws_bytes, norm_bwd_ws(Bp, L.out));
+        return hipSuccess;
+    };
+    for (auto* chain : {&w->enc, &w->dec})
+        for (auto& L : *chain)
+            if ((er = norm_bufs(L)) != hipSuccess) return er;
+    if (e->cfg.n_labels > 0) {
+        WA(w->Zl, Bp * K);
+        w->op_ws_bytes = std::max(w->op_ws_bytes, emb_bwd_ws(Bp, K));
+    }
+    if (w->op_ws_bytes > 0 && (er = hipMalloc(&w->op_ws, (size_t)w->op_ws_bytes)) != hipSuccess) return er;
 #undef WA
     const float one = 1.f;
     if ((er = hipMemcpy(w->one, &one, sizeof(float), hipMemcpyHostToDevice)) != hipSuccess) return er;
@@ -2336,10 +2371,12 @@ void wide_destroy(Engine* e) {
                      w->Mn, w->Z, w->Ep, w->dZ, w->dM, w->dA, w->Hn, w->dHn, w->NMr, w->NAr, w->Zn, w->En, w->dZn,
                      w->dNM, w->dNA, w->dT0, w->dT1, w->wtil, w->lossv})
         if (p) hipFree(p);
-    for (auto& L : w->enc)
-        if (L.act) hipFree(L.act);
-    for (auto& L : w->dec)
-        if (L.act) hipFree(L.act);
+    for (auto* chain : {&w->enc, &w->dec})
+        for (auto& L : *chain)
+            for (float* p : {L.act, L.lin, L.mean, L.rstd})
+                if (p) hipFree(p);
+    if (w->op_ws) hipFree(w->op_ws);
+    if (w->Zl) hipFree(w->Zl);
     if (w->pl_F) hipFree(w->pl_F);
     if (w->pl_E) hipFree(w->pl_E);
     delete w;
@@ -2396,6 +2433,15 @@ wide_poison_t wide_poison_bufs(Engine* e) {
     for (auto& L : w->enc) v.push_back({L.act, sizeof(float) * (size_t)(Bp * L.out)});
     for (auto& L : w->dec)
         if (L.act) v.push_back({L.act, sizeof(float) * (size_t)(Bp * L.out)});
+    for (auto* chain : {&w->enc, &w->dec})
+        for (auto& L : *chain)
+            if (L.lin) {
+                v.push_back({L.lin, sizeof(float) * (size_t)(Bp * L.out)});
+                v.push_back({L.mean, sizeof(float) * (size_t)Bp});
+                v.push_back({L.rstd, sizeof(float) * (size_t)Bp});
+            }
+    if (w->op_ws) v.push_back({w->op_ws, (size_t)w->op_ws_bytes});
+    if (w->Zl) v.push_back({w->Zl, sizeof(float) * (size_t)(Bp * K)});
     v.push_back({w->lossv, sizeof(float) * 8});
     return v;
 }
@@ -2451,10 +2497,83 @@ static GemmX enc_x(Engine* e) {
     return x;
 }
 
+// ---- norm and dropout of a layer (ops.hip), around its Linear ----
+static bool layer_in_norm(const WLayer& L) { return !L.norm.empty(); }
+// where the layer's Linear writes, and whether its epilogue applies the ReLU
+static float* layer_lin(const WLayer& L) { return layer_in_norm(L) ? L.lin : L.act; }
+static bool layer_gemm_relu(const WLayer& L) { return L.relu && !layer_in_norm(L); }
+static mmvae_norm_args layer_norm_args(Engine* e, const WLayer& L, int B, bool train) {
+    static_assert(offsetof(StepScalars, step_id) == 0 && offsetof(StepScalars, row_offset) == 8, "the dropout state");
+    mmvae_norm_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.M = B;
+    a.N = L.out;
+    a.x = L.lin;
+    a.ldx = a.ldy = a.lddy = a.lddx = L.out;
+    a.w = e->preg(L.norm + ".weight");
+    a.b = e->preg(L.norm + ".bias");
+    a.mean = L.mean;
+    a.rstd = L.rstd;
+    a.eps = 1e-5f;
+    a.relu = L.relu ? 1 : 0;
+    a.p = train && L.drop ? (double)e->cfg.dropout : 0.;
+    a.seed = L.seed;
+    a.state = reinterpret_cast<const int64_t*>(e->d_ss);  // step_id, row_offset
+    a.dtype = a.wtype = MMVAE_T_F32;
+    return a;
+}
+static mmvae_dropout_args layer_drop_args(Engine* e, const WLayer& L, int B, float* x) {
+    mmvae_dropout_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.M = B;
+    a.N = a.ldx = a.ldy = L.out;
+    a.x = a.y = x;
+    a.p = (double)e->cfg.dropout;
+    a.seed = L.seed;
+    a.state = reinterpret_cast<const int64_t*>(e->d_ss);
+    a.dtype = MMVAE_T_F32;
+    return a;
+}
+// behind the Linear: act = drop(relu?(norm(lin))), or dropout of act in place
+static hipError_t layer_fwd(Engine* e, const WLayer& L, int B, bool train) {
+    if (layer_in_norm(L)) {
+        ScopedTimer tm(e, "w_norm");
+        mmvae_norm_args a = layer_norm_args(e, L, B, train);
+        a.y = L.act;
+        return norm_fwd(a, e->stream);
+    }
+    if (!L.drop || !train) return hipSuccess;
+    ScopedTimer tm(e, "w_dropout");
+    return dropout(layer_drop_args(e, L, B, L.act), e->stream);
+}
+// the gradient at the layer's output -> at its Linear's output, in place
+static hipError_t layer_bwd(Engine* e, const WLayer& L, int B, float* d) {
+    if (layer_in_norm(L)) {
+        ScopedTimer tm(e, "w_norm_bwd");
+        mmvae_norm_args a = layer_norm_args(e, L, B, true);
+        a.dy = a.dx = d;
+        a.dw = e->greg(L.norm + ".weight");
+        a.db = e->greg(L.norm + ".bias");
+        a.ws = e->wide_st->op_ws;
+        a.ws_bytes = e->wide_st->op_ws_bytes;
+        return norm_bwd(a, e->stream);
+    }
+    if (L.drop) {
+        ScopedTimer tm(e, "w_dropout");
+        const hipError_t er = dropout(layer_drop_args(e, L, B, d), e->stream);
+        if (er != hipSuccess) return er;
+    }
+    if (L.relu) {  // (act is 0 where it was dropped too: so is d)
+        const int64_t n = (int64_t)B * L.out;
+        hipLaunchKernelGGL(k_w_relu_bwd, dim3(grid_for(n)), dim3(256), 0, e->stream, n, (const float*)L.act, d);
+    }
+    return hipGetLastError();
+}
+
 // the encoder chain from the raw batch X to the heads' input; returns it.  The first Linear
 // takes enc_in(X) (nb.hh:408-410 / vmf.hh:253-257): on bf16 / x3 handles transformed inside the
 // GEMM, on f32 handles from the materialised block Xn (the exact f32 GEMM)
-static const float* enc_forward(Engine* e, int B, hipError_t& er) {
+static const float* enc_forward(Engine* e, int B, bool train, hipError_t& er) {
     WideState* w = e->wide_st;
     const GemmX gx = enc_x(e);
     const float* x = nullptr;
@@ -2465,8 +2584,8 @@ static const float* enc_forward(Engine* e, int B, hipError_t& er) {
         g.M = B; g.N = L.out; g.K = L.in;
         g.sam = ld; g.sak = 1;
         g.B = L.W; g.sbk = 1; g.sbn = L.in;
-        g.C = L.act; g.scm = L.out; g.scn = 1;
-        g.bias = L.b; g.act = L.relu ? 1 : 0;
+        g.C = layer_lin(L); g.scm = L.out; g.scn = 1;
+        g.bias = L.b; g.act = layer_gemm_relu(L) ? 1 : 0;
         if (l == 0 && at_in_gemm(e)) {
             g.A = w->X;
             er = gemm(e, g, &gx);
@@ -2480,6 +2599,7 @@ static const float* enc_forward(Engine* e, int B, hipError_t& er) {
             g.A = x;
             er = gemm(e, g);
         }
+        if (er == hipSuccess) er = layer_fwd(e, L, B, train);
         if (er != hipSuccess) return nullptr;
         x = L.act;
         ld = L.out;
@@ -2605,10 +2725,7 @@ static hipError_t enc_backward(Engine* e, int B, const ColOut& o) {
     for (int l = (int)w->enc.size() - 1; l >= 0; --l) {
         const WLayer& L = w->enc[l];
         hipError_t er;
-        if (L.relu) {
-            hipLaunchKernelGGL(k_w_relu_bwd, dim3(grid_for((int64_t)B * L.out)), dim3(256), 0, e->stream,
-                               (int64_t)B * L.out, (const float*)L.act, cur);
-        }
+        if ((er = layer_bwd(e, L, B, cur)) != hipSuccess) return er;
         if (l > 0) {
             if ((er = linear_dx(e, B, L.out, L.in, cur, L.out, L.W, nxt, L.in)) != hipSuccess) return er;
             std::swap(cur, nxt);
@@ -2643,15 +2760,39 @@ static hipError_t enc_backward(Engine* e, int B, const ColOut& o) {
     return hipGetLastError();
 }
 
-// decoder chain forward from z [B][K] to the last hidden output; returns the final layer's input
+// the batch's labels (staged in the permutation's place) as an embedding call
+static mmvae_embedding_args label_args(Engine* e, int B) {
+    mmvae_embedding_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.T = B;
+    a.N = e->K;
+    a.V = e->cfg.n_labels;
+    a.ids = e->d_perm;
+    a.dtype = MMVAE_T_F32;
+    a.scale = e->cfg.label_scale;
+    return a;
+}
+// decoder chain forward from z [B][K] (with labels: z + label_scale E[label]) to the last hidden
+// output; returns the final layer's input
 static const float* dec_hidden_fwd(Engine* e, int B, hipError_t& er) {
     WideState* w = e->wide_st;
     const float* x = w->Z;
     int64_t ld = e->K;
+    if (w->Zl) {
+        ScopedTimer tm(e, "w_embed");
+        mmvae_embedding_args a = label_args(e, B);
+        a.table = e->preg("label_embedding.weight");
+        a.add = w->Z;
+        a.y = w->Zl;
+        a.ldt = a.ldadd = a.ldy = e->K;
+        if ((er = emb_fwd(a, e->stream)) != hipSuccess) return nullptr;
+        x = w->Zl;
+    }
     for (size_t l = 0; l + 1 < w->dec.size(); ++l) {
         WLayer& L = w->dec[l];
-        if ((er = linear_fwd(e, B, L.out, L.in, x, ld, L.W, L.b, L.act, L.out, L.relu ? 1 : 0)) != hipSuccess)
+        if ((er = linear_fwd(e, B, L.out, L.in, x, ld, L.W, L.b, layer_lin(L), L.out, layer_gemm_relu(L) ? 1 : 0)) != hipSuccess)
             return nullptr;
+        if ((er = layer_fwd(e, L, B, true)) != hipSuccess) return nullptr;
         x = L.act;
         ld = L.out;
     }
@@ -2669,12 +2810,20 @@ static hipError_t dec_backward(Engine* e, int B) {
     float *cur = w->dT0, *nxt = w->dT1;
     for (int l = nl - 2; l >= 0; --l) {
         const WLayer& L = w->dec[l];
-        if (L.relu)
-            hipLaunchKernelGGL(k_w_relu_bwd, dim3(grid_for((int64_t)B * L.out)), dim3(256), 0, e->stream,
-                               (int64_t)B * L.out, (const float*)L.act, cur);
+        if ((er = layer_bwd(e, L, B, cur)) != hipSuccess) return er;
         float* d = (l == 0) ? w->dZ : nxt;
         if ((er = linear_dx(e, B, L.out, L.in, cur, L.out, L.W, d, L.in)) != hipSuccess) return er;
         std::swap(cur, nxt);
+    }
+    if (w->Zl) {  // dE from the gradient at z + label_scale E[label], which is also dz
+        ScopedTimer tm(e, "w_embed_bwd");
+        mmvae_embedding_args a = label_args(e, B);
+        a.dy = w->dZ;
+        a.lddy = e->K;
+        a.dtable = e->greg("label_embedding.weight");
+        a.ws = w->op_ws;
+        a.ws_bytes = w->op_ws_bytes;
+        if ((er = emb_bwd(a, e->stream)) != hipSuccess) return er;
     }
     return hipGetLastError();
 }
@@ -2729,7 +2878,7 @@ static hipError_t nb_step(Engine* e, int B, int64_t n_total, float beta, bool up
     hipLaunchKernelGGL(k_w_gene, dim3((D + 255) / 256), dim3(256), 0, e->stream, D, (const float*)e->preg("ln_x_sd"),
                        1e-4f, w->gvec);
     hipError_t er = hipSuccess;
-    const float* h = enc_forward(e, B, er);
+    const float* h = enc_forward(e, B, true, er);
     WCHK(er);
     WCHK(heads_fwd(e, B, h, "mu_representation_mean", "mu_representation_logvariance", true));
     // overdispersion encoder on raw x (nb.hh:444-451)
@@ -2910,7 +3059,7 @@ static hipError_t vmf_step(Engine* e, int B, int64_t n_total, float beta, bool u
     hipLaunchKernelGGL(k_w_gene, dim3((D + 255) / 256), dim3(256), 0, e->stream, D, (const float*)e->preg("ln_x_sd"),
                        epsD, w->gvec);
     hipError_t er = hipSuccess;
-    const float* h = enc_forward(e, B, er);
+    const float* h = enc_forward(e, B, true, er);
     WCHK(er);
     WCHK(heads_fwd(e, B, h, "representation_mean", "representation_logvariance", true));
     WLat la;
@@ -3004,7 +3153,7 @@ hipError_t wide_encode(Engine* e, int64_t B, float* d_mean, float* d_lnvar) {
     hipLaunchKernelGGL(k_w_gene, dim3((D + 255) / 256), dim3(256), 0, e->stream, D, (const float*)e->preg("ln_x_sd"),
                        vmf ? epsD : 1e-4f, w->gvec);
     hipError_t er = hipSuccess;
-    const float* h = enc_forward(e, (int)B, er);
+    const float* h = enc_forward(e, (int)B, false, er);
     WCHK(er);
     if (vmf) WCHK(heads_fwd(e, (int)B, h, "representation_mean", "representation_logvariance", false));
     else WCHK(heads_fwd(e, (int)B, h, "mu_representation_mean", "mu_representation_logvariance", false));

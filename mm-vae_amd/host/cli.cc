@@ -3,7 +3,8 @@
 // ignored (opterr = 0): mmvae options (mmvae.hh:68-209), training options (mmvae_alg.hh:36-125),
 // then the model's (nb.hh:73-194 / vmf.hh:75-186) — a short option therefore means one thing
 // per group, and this parser keeps exactly that behaviour.  A fourth group holds the engine's
-// own options (--seed, --dtype, --device, --threads, --no_csr_cache, --verbose).
+// own options (--seed, --dtype, --device, --threads, --no_csr_cache, --verbose, and the layer chains'
+// --layer_norm, --dropout, --labels, --label_scale).
 //
 // Outputs as the reference: ${out}.scores.gz (per-epoch loss), ${out}.covar.mtx.gz (+ .index) when
 // --covar is absent (create_ones_like), ${mtx}.index when missing (BGZF inputs), recorder files
@@ -17,6 +18,7 @@
 #include <unistd.h>
 
 #include <chrono>
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -83,7 +85,15 @@ int parse_options(int argc, const char** argv, int model, CliOptions& o) {
     static const option en_long[] = {{"seed", required_argument, nullptr, 1},      {"dtype", required_argument, nullptr, 2},
                                      {"device", required_argument, nullptr, 3},    {"threads", required_argument, nullptr, 4},
                                      {"no_csr_cache", no_argument, nullptr, 5},    {"verbose", no_argument, nullptr, 6},
-                                     {"quiet", no_argument, nullptr, 7},           {nullptr, no_argument, nullptr, 0}};
+                                     {"quiet", no_argument, nullptr, 7},           {"layer_norm", no_argument, nullptr, 8},
+                                     {"dropout", required_argument, nullptr, 9},   {"labels", required_argument, nullptr, 10},
+                                     {"label_scale", required_argument, nullptr, 11}, {nullptr, no_argument, nullptr, 0}};
+    bool numbers = true;
+    auto number = [&](const std::string& v, float& x) {
+        char* end = nullptr;
+        x = std::strtof(v.c_str(), &end);
+        numbers = numbers && end != v.c_str() && *end == 0;
+    };
     mmvae_opt_detail::each_opt(argc, argv, "", en_long, [&](int c, const std::string& v) {
         switch (c) {
             case 1: o.seed = std::stoull(v); break;
@@ -93,6 +103,10 @@ int parse_options(int argc, const char** argv, int model, CliOptions& o) {
             case 5: o.csr_cache = false; break;
             case 6: o.verbose = true; break;
             case 7: o.verbose = false; break;
+            case 8: o.layer_norm = true; break;
+            case 9: number(v, o.dropout); break;
+            case 10: o.labels = v; break;
+            case 11: number(v, o.label_scale); break;
             default: break;
         }
         return false;
@@ -101,6 +115,10 @@ int parse_options(int argc, const char** argv, int model, CliOptions& o) {
     if (o.covar_idx.empty()) o.covar_idx = o.covar_mtx + ".index";
     if (dtype_code(o.dtype) < 0) {
         std::fprintf(stderr, "unknown --dtype %s (f32 | bf16x3 | bf16 | fp8)\n", o.dtype.c_str());
+        return MMVAE_E_ARG;
+    }
+    if (!numbers || !(o.dropout >= 0.f && o.dropout < 1.f) || !std::isfinite(o.label_scale)) {
+        std::fprintf(stderr, "--dropout needs a number in [0, 1), --label_scale a finite number\n");
         return MMVAE_E_ARG;
     }
     return MMVAE_OK;
@@ -120,11 +138,13 @@ const char* usage_text(int model) {
                ? "nb_vae_main --mtx X.mtx.gz --out OUT [--batch_size 100 --max_epoch 101 --nboot 3 --lr 1e-3\n"
                  "             --mean_latent 2 --overdisp_encoding 1 --overdispersion_latent 1 --kl_discount .1\n"
                  "             --kl_max 1 --kl_min .01 --recording 10 --covar C.mtx.gz]\n"
-                 "engine: [--dtype f32|bf16x3|bf16|fp8 --seed S --device G --threads T --no_csr_cache --verbose]\n"
+                 "engine: [--dtype f32|bf16x3|bf16|fp8 --seed S --device G --threads T --no_csr_cache --verbose\n"
+                 "         --layer_norm --dropout 0 --labels L.txt.gz --label_scale 1]\n"
                : "vmf_vae_main --mtx X.mtx.gz --out OUT [--batch_size 100 --max_epoch 101 --nboot 3 --lr 1e-3\n"
                  "             --latent 2 --kappa_min .1 --kappa_max 10 --kl_discount .1 --kl_max 1 --kl_min .01\n"
                  "             --recording 10 --covar C.mtx.gz]\n"
-                 "engine: [--dtype f32|bf16x3|bf16 --seed S --device G --threads T --no_csr_cache --verbose]\n"
+                 "engine: [--dtype f32|bf16x3|bf16 --seed S --device G --threads T --no_csr_cache --verbose\n"
+                 "         --layer_norm --dropout 0 --labels L.txt.gz --label_scale 1]\n"
                  "        (fp8 is built for the NB model only)\n";
 }
 
@@ -284,8 +304,24 @@ int run_cli(int argc, const char** argv, int model) {
             ensure_index(f, f + ".index", o.verbose);
         }
     }
+    // labels (not in the reference): one per cell, the decoder's learned vector of each
+    std::vector<int32_t> labels;
+    int64_t n_labels = 0;
+    if (!o.labels.empty()) {
+        int32_t* l = nullptr;
+        if (mmvae_labels_read(o.labels.c_str(), csr.N, &l, &n_labels)) {
+            std::fprintf(stderr, "%s\n", mmvae_host_last_error());
+            return EXIT_FAILURE;
+        }
+        labels.assign(l, l + csr.N);
+        mmvae_free(l);
+    }
     mmvae_cfg cfg;
     mmvae_cfg_default(&cfg, model);
+    cfg.layer_norm = o.layer_norm ? 1 : 0;
+    cfg.dropout = o.dropout;
+    cfg.n_labels = n_labels;
+    cfg.label_scale = o.label_scale;
     cfg.dtype = dtype_code(o.dtype);
     cfg.D = csr.D;
     cfg.C = C;
@@ -309,6 +345,7 @@ int run_cli(int argc, const char** argv, int model) {
     }
     int rc = mmvae_upload_csr(h, csr.rowptr, csr.col, csr.val, csr.N, csr.D, covar.empty() ? nullptr : covar.data());
     mmvae_csr_free(&csr);
+    if (!rc && n_labels > 0) rc = mmvae_set_labels(h, labels.data(), (int64_t)labels.size());
     if (!rc) rc = mmvae_init_params(h, o.seed);
     // one hipGraph per step shape (single-rank runs; with a communicator the steps stay eager)
     if (!rc && !std::getenv("MMVAE_NO_GRAPH")) rc = mmvae_graph_enable(h, 1);

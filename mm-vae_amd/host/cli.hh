@@ -29,6 +29,10 @@ struct CliOptions {
     int device = -1;
     int threads = 0;
     bool csr_cache = true;
+    bool layer_norm = false;  // --layer_norm: the hidden chains' layers normalised (mmvae_cfg.layer_norm)
+    float dropout = 0.f;      // --dropout
+    std::string labels;       // --labels: the cells' label file (mmvae_labels_read)
+    float label_scale = 1.f;  // --label_scale
     bool verbose = true;
     bool help = false;
     int mm_rc = 0;  // parse_mmvae_options' result (EXIT_FAILURE: missing mtx / out)

@@ -1261,6 +1261,45 @@ int mmvae_mtx_write_csr(const char* path, const mmvae_csr* c) {
     return w.close() ? MMVAE_OK : fail(MMVAE_E_ARG, std::string("write failed: ") + path);
 }
 
+int mmvae_labels_read(const char* path, int64_t N, int32_t** labels, int64_t* n_labels) {
+    if (!path || !labels || !n_labels || N < 1) return fail(MMVAE_E_ARG, "labels_read: bad arguments");
+    gzFile f = gzopen(path, "rb");  // (reads plain text too)
+    if (!f) return fail(MMVAE_E_ARG, std::string("cannot read ") + path);
+    int32_t* out = static_cast<int32_t*>(std::malloc(sizeof(int32_t) * (size_t)N));
+    int64_t i = 0, top = -1;
+    std::string wrong = out ? "" : "out of host memory";
+    char line[256];
+    while (wrong.empty() && gzgets(f, line, sizeof(line))) {
+        size_t n = std::strlen(line);
+        while (n > 0 && std::strchr(" \t\r\n", line[n - 1])) line[--n] = 0;
+        const char* at = line + std::strspn(line, " \t");
+        char* end = nullptr;
+        errno = 0;
+        const long long v = std::strcmp(at, "NA") == 0 ? -1 : std::strtoll(at, &end, 10);
+        if (i == N) {
+            wrong = "more lines than the " + std::to_string(N) + " cells";
+        } else if ((end && (end == at || *end)) || errno || v < -1 || v > INT32_MAX - 65536) {
+            wrong = "line " + std::to_string(i + 1) + " is not a label (a whole number >= 0, -1 or NA)";
+        } else {
+            out[i++] = (int32_t)v;
+            top = std::max<int64_t>(top, v);
+        }
+    }
+    if (wrong.empty() && i < N) wrong = std::to_string(i) + " labels for " + std::to_string(N) + " cells";
+    int zerr = Z_OK;
+    (void)gzerror(f, &zerr);
+    if (wrong.empty() && zerr < 0) wrong = "the file is damaged";
+    gzclose(f);
+    if (wrong.empty() && top < 0) wrong = "no cell has a label";
+    if (!wrong.empty()) {
+        std::free(out);
+        return fail(MMVAE_E_ARG, std::string(path) + ": " + wrong);
+    }
+    *labels = out;
+    *n_labels = top + 1;
+    return MMVAE_OK;
+}
+
 int mmvae_mtx_write_ones(const char* path, int64_t N) {
     if (!path || N < 1) return fail(MMVAE_E_ARG, "mtx_write_ones: bad arguments");
     BgzfWriter w;

@@ -38,7 +38,8 @@ class Cfg(ctypes.Structure):
                 ("grad_clip", ctypes.c_float), ("kappa_min", ctypes.c_float), ("kappa_max", ctypes.c_float),
                 ("seed", ctypes.c_uint64), ("relu", ctypes.c_int32), ("n_enc_hidden", ctypes.c_int32),
                 ("n_dec_hidden", ctypes.c_int32), ("enc_hidden", ctypes.c_int32 * MAX_HIDDEN),
-                ("dec_hidden", ctypes.c_int32 * MAX_HIDDEN)]
+                ("dec_hidden", ctypes.c_int32 * MAX_HIDDEN), ("layer_norm", ctypes.c_int32), ("dropout", ctypes.c_float),
+                ("n_labels", ctypes.c_int64), ("label_scale", ctypes.c_float), ("reserved", ctypes.c_int32)]
 
 
 class StepArgs(ctypes.Structure):
@@ -69,6 +70,7 @@ def lib():
         "mmvae_upload_csr": (ctypes.c_int, [h, i64p, ctypes.POINTER(ctypes.c_int32), f32p, i64, i64, f32p]),
         "mmvae_synth_csr": (ctypes.c_int, [h, i64, ctypes.c_double, ctypes.c_uint64, i64p]),
         "mmvae_stream_csr": (ctypes.c_int, [h, i64p, ctypes.POINTER(ctypes.c_int32), f32p, i64, i64, f32p]),
+        "mmvae_set_labels": (ctypes.c_int, [h, ctypes.POINTER(ctypes.c_int32), i64]),
         "mmvae_dataset_size": (ctypes.c_int, [h, i64p, i64p]),
         "mmvae_param_shape": (ctypes.c_int, [h, i32, ctypes.POINTER(i32), i64p]),
         "mmvae_comm_allreduce": (ctypes.c_int, [h, f32p, i64]),
@@ -136,7 +138,10 @@ class Engine:
     """One model + optimiser + HBM dataset on one GPU (the C handle)."""
 
     def __init__(self, D, K, C=1, H=1, R=1, max_batch=100, dtype="f32", model=MODEL_NB, device=0, seed=42,
-                 lr=1e-3, kappa_min=0.1, kappa_max=10.0, relu=False, enc_hidden=(), dec_hidden=()):
+                 lr=1e-3, kappa_min=0.1, kappa_max=10.0, relu=False, enc_hidden=(), dec_hidden=(), layer_norm=False,
+                 dropout=0.0, n_labels=0, label_scale=1.0):
+        """layer_norm, dropout: after every layer of the encoder chain and every hidden layer of the decoder's;
+        n_labels: the decoder reads z + label_scale * label_embedding.weight[label] (:meth:`set_labels`)."""
         L = lib()
         c = default_cfg(model)
         c.D, c.K, c.C, c.H, c.R, c.max_batch = D, K, C, H, R, max_batch
@@ -150,6 +155,7 @@ class Engine:
             c.dec_hidden[i] = int(v)
         c.dtype = _DTYPES[dtype] if isinstance(dtype, str) else int(dtype)
         c.seed, c.lr, c.kappa_min, c.kappa_max = seed, lr, kappa_min, kappa_max
+        c.layer_norm, c.dropout, c.n_labels, c.label_scale = 1 if layer_norm else 0, dropout, n_labels, label_scale
         self.cfg = c
         self.D, self.K, self.C, self.H, self.R = D, K, C, H, R
         self.max_batch = max_batch
@@ -207,6 +213,14 @@ class Engine:
         self._chk(lib().mmvae_synth_csr(self._h, N, lib_size, seed, ctypes.byref(nnz)), "synth_csr")
         self.N = N
         return nnz.value
+
+    def set_labels(self, labels):
+        """The dataset cells' labels [N]: 0 .. n_labels - 1, or -1 (mmvae_set_labels; after the dataset)."""
+        a = np.asarray(labels)
+        lab = np.ascontiguousarray(a, dtype=np.int32)
+        if not np.array_equal(lab, a):
+            raise MMVAEError("labels must be whole numbers below 2^31")
+        self._chk(lib().mmvae_set_labels(self._h, _ptr(lab, ctypes.c_int32), lab.size), "set_labels")
 
     def get_rows(self, rows):
         rows = np.ascontiguousarray(rows, dtype=np.int64)

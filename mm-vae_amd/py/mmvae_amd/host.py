@@ -52,6 +52,7 @@ def hlib():
                                                   ctypes.POINTER(i64), ctypes.POINTER(ctypes.POINTER(ctypes.c_float))]),
         "mmvae_free": (None, [ctypes.c_void_p]),
         "mmvae_mtx_write_ones": (ctypes.c_int, [ctypes.c_char_p, i64]),
+        "mmvae_labels_read": (ctypes.c_int, [ctypes.c_char_p, i64, ctypes.POINTER(ctypes.POINTER(ctypes.c_int32)), ctypes.POINTER(i64)]),
         "mmvae_mtx_build_index": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_char_p]),
         "mmvae_mtx_read_index": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(ctypes.POINTER(i64)),
                                                 ctypes.POINTER(i64)]),
@@ -95,6 +96,15 @@ def mtx_read(path, threads=0):
     if rc:
         _err("mtx_read", rc)
     return _take(c)
+
+
+def labels_read(path, N):
+    """A label file (one per cell and line, -1 or NA: none) -> (labels int32 [N], n_labels)."""
+    p, n = ctypes.POINTER(ctypes.c_int32)(), ctypes.c_int64()
+    rc = hlib().mmvae_labels_read(os.fsencode(path), N, ctypes.byref(p), ctypes.byref(n))
+    if rc:
+        _err("labels_read", rc)
+    return _owned(p, N), n.value
 
 
 def csr_save(path, rowptr, col, val, D):

@@ -4,8 +4,9 @@ The reference has no such layers; these are the definitions the operators' docum
 the error bounds that 32-bit evaluation of them has."""
 import numpy as np
 import torch
+import torch.nn.functional as F
 
-from . import philox
+from . import nb_oracle, philox, vmf_oracle
 
 U32 = 2.0 ** -24  # half a step of float32, relative
 
@@ -99,3 +100,61 @@ def embedding_grad(dy, ids, rows, scale):
     out = torch.zeros(rows + 1, d.shape[1]).double().index_add_(0, i, d)
     mag = torch.zeros(rows + 1, d.shape[1]).double().index_add_(0, i, d.abs())
     return out[:rows] * scale, 130 * U32 * abs(scale) * mag[:rows]
+
+
+# ---- the models with normalised, dropped-out, label-conditioned layer chains --------------------
+class _Chains:
+    """The layer chains of a model oracle with cfg.layer_norm / dropout / n_labels.  `key` = (seed, step,
+    row_offset) of the step; params hold the norms' weights and the label table under their names."""
+    layer_norm, dropout, label_scale, labels, key, training = False, 0.0, 1.0, None, (42, 0, 0), True
+
+    def _after(self, x, seq, l, relu):
+        seed, step, ro = self.key
+        if self.layer_norm:
+            n = f"{self.prefix}{seq}.norm_{l + 1}"
+            x = F.layer_norm(x, (x.shape[1],), self.p[n + ".weight"], self.p[n + ".bias"], 1e-5)
+        if relu:
+            x = F.relu(x)
+        if self.dropout > 0 and self.training:
+            k = seed + 0x9E3779B97F4A7C15 * ((1 if seq == "enc" else 101) + l)
+            x = x * drop_factor(*x.shape, float(np.float32(self.dropout)), k, step, ro).to(x.dtype)
+        return x
+
+    def _z(self, z):
+        if self.labels is None:
+            return z
+        t = self.p["label_embedding.weight"]
+        ok = (self.labels >= 0)[:, None]
+        return z + self.label_scale * torch.where(ok, t[self.labels.clamp(min=0)], torch.zeros_like(z))
+
+
+class NBLayers(_Chains, nb_oracle.NBModel):
+    prefix = "mu_"
+
+    def _seq(self, keys, x, final_relu):
+        enc = keys is self.enc_keys
+        if not enc:
+            x = self._z(x)
+        for i, k in enumerate(keys):
+            x = F.linear(x, self.fr[k + ".weight"], self.fr[k + ".bias"])
+            last = i == len(keys) - 1
+            if enc or not last:
+                x = self._after(x, "enc" if enc else "dec", i, self.relu and (not last or final_relu))
+        return x
+
+
+class VMFLayers(_Chains, vmf_oracle.VMFModel):
+    prefix = "z_"
+
+    def z_enc(self, x):
+        for i, k in enumerate(self.enc_keys):
+            x = self._after(self.angular(x, k), "enc", i, self.relu)
+        return x
+
+    def z_dec(self, z):
+        z = self._z(z)
+        for i, k in enumerate(self.dec_keys):
+            z = F.linear(z, self.fr[k + ".weight"], self.fr[k + ".bias"])
+            if i < len(self.dec_keys) - 1:
+                z = self._after(z, "dec", i, self.relu)
+        return z

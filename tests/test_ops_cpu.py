@@ -1,7 +1,7 @@
 """CPU tests of the layer operators' boundary (include/mmvae_capi.h, mmvae_amd.ops): the packed argument
 structs match the header's, every wrong call is refused before a device is touched, the oracle's own
 formulas hold against differences, and the dropout masks have the stated rate."""
-import ctypes
+import gzip
 import os
 import re
 import subprocess
@@ -11,7 +11,7 @@ import pytest
 import torch
 
 import mmvae_amd
-from mmvae_amd import ops
+from mmvae_amd import host, ops
 from oracle import layers
 
 INCLUDE = os.path.dirname(mmvae_amd.HEADER_PATH)
@@ -187,3 +187,44 @@ def test_dropout_rate_and_independence(p):
             assert abs(agree - (q * q + (1 - q) ** 2)) < 0.02
     # a shard's rows are the whole batch's
     assert torch.equal(layers.drop_kept(50, N, p, 123, 4, row_offset=100), k[100:150])
+
+
+@pytest.mark.parametrize("kw,msg", [(dict(dropout=-0.1), "dropout"), (dict(dropout=1.0), "dropout"), (dict(dropout=float("nan")), "dropout"),
+                                    (dict(n_labels=-1), "n_labels"), (dict(n_labels=2 ** 31), "n_labels"), (dict(n_labels=2, label_scale=float("inf")), "label_scale"),
+                                    (dict(layer_norm=True, relu=True, enc_hidden=(8,)), "mu_encoding_1")])
+def test_engine_layer_options_refused(kw, msg):
+    with pytest.raises(mmvae_amd.MMVAEError, match=msg):
+        mmvae_amd.Engine(D=10, K=4, **kw)
+
+
+def test_label_files(tmp_path):
+    f = tmp_path / "l.txt"
+    f.write_text("0\n 3 \nNA\n-1\n1")
+    lab, n = host.labels_read(f, 5)
+    assert lab.tolist() == [0, 3, -1, -1, 1] and n == 4
+    g = tmp_path / "l.gz"
+    g.write_bytes(gzip.compress(b"7\n" * 5))
+    assert host.labels_read(g, 5)[1] == 8
+    for text, msg in (("0\n1\n", "2 labels for 5"), ("0\n" * 6, "more lines"), ("0\n\n1\n1\n1\n", "line 2"), ("0\nx\n1\n1\n1\n", "line 2"), ("1.5\n", "line 1"),
+                      ("-2\n", "line 1"), ("9999999999\n", "line 1"), ("NA\n" * 5, "no cell"), ("", "0 labels")):
+        f.write_text(text)
+        with pytest.raises(mmvae_amd.MMVAEError, match=msg):
+            host.labels_read(f, 5)
+    g.write_bytes(gzip.compress(b"7\n" * 50000)[:-20])  # cut off
+    with pytest.raises(mmvae_amd.MMVAEError):
+        host.labels_read(g, 50000)
+    with pytest.raises(mmvae_amd.MMVAEError, match="cannot read"):
+        host.labels_read(tmp_path / "none", 5)
+
+
+@pytest.mark.parametrize("exe", ["nb_vae_main", "vmf_vae_main"])
+def test_cli_layer_options_refused(tmp_path, exe):
+    p = tmp_path / "x.mtx"
+    p.write_text("%%MatrixMarket matrix coordinate integer general\n3 2 2\n1 1 4\n3 2 1\n")
+    lab = tmp_path / "l.txt"
+    lab.write_text("0\n")
+    base = [os.path.join(host.BIN_DIR, exe), "--mtx", str(p), "--out", str(tmp_path / "o")]
+    for more, msg in ((["--dropout", "1.0"], "--dropout"), (["--dropout", "much"], "--dropout"), (["--label_scale", "inf"], "--label_scale"),
+                      (["--labels", str(lab)], "1 labels for 2"), (["--labels", str(tmp_path / "none")], "cannot read")):
+        r = subprocess.run(base + more, capture_output=True, text=True, timeout=60)
+        assert r.returncode == 1 and msg in r.stderr, (more, r.stderr)
