@@ -1,0 +1,621 @@
+// Layer norm, forward and backward (ops.hip's entries): the kernels and their launch for one type of
+// activations; each type is a translation unit of its own (norm_f32 / _bf16 / _f16.hip).
+#pragma once
+#include "ops_dev.hpp"
+
+namespace mmvae {
+
+// =======================================================================================
+// Layer norm over rows of N: y = drop(act(xh w + b)), xh = (x - mean) rstd
+// TPR threads hold a row (VPT chunks each) in registers: x is read once, the variance is the
+// mean square of the differences from the mean.
+// =======================================================================================
+struct NormP {
+    int64_t M;
+    int N;
+    const void *x, *w, *b, *dy;
+    int64_t ldx, lddy, ldy;  // ldy: of y, or of dx
+    void* y;                 // y, or dx
+    float *mean, *rstd;
+    float* part;             // backward: the workgroups' sums [grid][2][Np]; null: one workgroup writes
+    void *dw, *db;           //   dw / db (or there are none)
+    int64_t Np;
+    float eps;
+    int relu;
+    bool wf32;
+    bool b_lds;              // forward, weights in LDS: the biases too
+    DropKey drop;
+};
+
+// u = xh w + b, as forward and backward both compute it (the ReLU's side must be the same)
+MMVAE_DEV float ln_u(float x, float mean, float rstd, float w, float b) { return __builtin_fmaf((x - mean) * rstd, w, b); }
+
+// A thread's weights stay with it over its rows: in registers, or for rows of more than 8192 columns
+// (BLK = 1024) in LDS, where they leave the registers to the row.  Biases that do not fit there too
+// (N > 20,480) are read with every row.
+template <int BLK> struct LnHold {
+    static constexpr bool LDS = BLK == 1024;
+};
+static constexpr int LN_LDS = 163840;  // bytes of LDS of a CU
+
+// a pointer into LDS that the compiler takes for a new one: what is read there is read again (with every
+// row, in every phase) instead of being kept in registers from before
+MMVAE_DEV float* lds_anew(float* l) {
+    int zero = 0;
+    asm volatile("" : "+s"(zero));
+    return l + zero;
+}
+
+// MASK: with a ReLU or dropout
+template <class T, int TPR, int VPT, int BLK, bool MASK, bool EVEN>
+__global__ __launch_bounds__(BLK) void k_ln_fwd(NormP a) {
+    constexpr int RPB = BLK / TPR;
+    constexpr bool HOLD = !LnHold<BLK>::LDS;
+    extern __shared__ float4 dyn_lds[];
+    float* lw = reinterpret_cast<float*>(dyn_lds);
+    __shared__ float red[2][BLK / 64];
+    const int lane = threadIdx.x % TPR, grp = threadIdx.x / TPR;
+    const int N = a.N, slots = (N + 7) / 8;
+    const float inv = 1.f / (float)N;
+    if (MASK) drop_state(a.drop);
+    float hw[HOLD ? VPT : 1][8], hb[HOLD ? VPT : 1][8];
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        const int c = j * TPR + lane, col = c * 8;
+        ldw<T>(a.w, a.wf32, col, N - col, 1.f, hw[HOLD ? j : 0]);
+        if (HOLD || a.b_lds) ldw<T>(a.b, a.wf32, col, N - col, 0.f, hb[HOLD ? j : 0]);
+        if (!HOLD && c < slots) {
+            lds_put8(lw, slots, c, hw[0]);
+            if (a.b_lds) lds_put8(lw + slots * 8, slots, c, hb[0]);
+        }
+    }
+    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.M; r0 += (int64_t)gridDim.x * RPB) {
+        const int64_t row = r0 + grp;
+        const bool ok = row < a.M;
+        const T* xr = (const T*)a.x + (ok ? row : 0) * a.ldx;
+        Chunk<T> xc[VPT];
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int col = (j * TPR + lane) * 8;
+            xc[j] = ld_row<EVEN>(xr, col, N);
+        }
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            float t = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t += xc[j].get(i);
+            s += !EVEN || (j * TPR + lane) * 8 < N ? t : 0.f;
+        }
+        const float mean = row_sum<TPR>(s, red[0]) * inv;
+        float q = 0.f;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int n = N - (j * TPR + lane) * 8;
+            float t = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float d = EVEN || i < n ? xc[j].get(i) - mean : 0.f;
+                t = __builtin_fmaf(d, d, t);
+            }
+            q += !EVEN || n > 0 ? t : 0.f;
+        }
+        const float rstd = 1.f / sqrtf(row_sum<TPR>(q, red[1]) * inv + a.eps);
+        if (ok) {
+            T* yr = (T*)a.y + row * a.ldy;
+            const float* rw = HOLD ? lw : lds_anew(lw);
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                const int c = j * TPR + lane, col = c * 8, n = N - col;
+                if (n <= 0) continue;
+                float w[8], b[8];
+                if constexpr (!HOLD) {
+                    lds_get8(rw, slots, c, w);
+                    if (a.b_lds) lds_get8(rw + slots * 8, slots, c, b);
+                    else ldw<T>(a.b, a.wf32, col, n, 0.f, b);
+                }
+                float u[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    u[i] = ln_u(xc[j].get(i), mean, rstd, HOLD ? hw[HOLD ? j : 0][i] : w[i], HOLD ? hb[HOLD ? j : 0][i] : b[i]);
+                if (MASK && a.relu) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) u[i] = u[i] > 0.f || u[i] != u[i] ? u[i] : 0.f;  // (a NaN stays one)
+                }
+                if (MASK && a.drop.thr) {
+                    bool kept[8];
+                    keep8(a.drop, row, c, kept);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) u[i] = kept[i] ? u[i] * a.drop.s : 0.f;
+                }
+                Chunk<T> yc;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) yc.set(i, u[i]);
+                if constexpr (EVEN) yc.store(yr + col);
+                else st8(yr + col, n, yc);
+            }
+            if (lane == 0) {
+                if (a.mean) a.mean[row] = mean;
+                if (a.rstd) a.rstd[row] = rstd;
+            }
+        }
+        if constexpr (TPR > 64) __syncthreads();  // the next row's sums reuse `red`
+    }
+}
+
+// backward: du = dy m [u > 0], g = du w, dx = rstd (g - mean(g) - xh mean(g xh)); the workgroup's
+// sums of du xh and du over its rows (fixed order: a thread's rows, then the row groups) -> part, or
+// with one workgroup straight into dw / db.  Elements behind a row's end are loaded as 0 and add 0.
+template <class T, int TPR, int VPT, int BLK, bool MASK, bool EVEN>
+__global__ __launch_bounds__(BLK, BLK / 256) void k_ln_bwd(NormP a) {
+    constexpr int RPB = BLK / TPR;
+    constexpr bool HOLD = !LnHold<BLK>::LDS || TPR <= 64, AGAIN = VPT >= 3 && (MASK || VPT == 4 || sizeof(T) == 4);
+    extern __shared__ float4 dyn_lds[];
+    float* lw = reinterpret_cast<float*>(dyn_lds);
+    __shared__ float red[2][BLK / 64];
+    const int lane = threadIdx.x % TPR, grp = threadIdx.x / TPR;
+    const int N = a.N, slots = (N + 7) / 8;
+    const float inv = 1.f / (float)N, ds = MASK && a.drop.thr ? a.drop.s : 1.f;
+    if (MASK) drop_state(a.drop);
+    float hw[HOLD ? VPT : 1][8];
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        const int c = j * TPR + lane, col = c * 8;
+        ldw<T>(a.w, a.wf32, col, N - col, 1.f, hw[HOLD ? j : 0]);
+        if (!HOLD && c < slots) lds_put8(lw, slots, c, hw[0]);
+    }
+    float aw[VPT][8], ab[VPT][8];
+#pragma unroll
+    for (int j = 0; j < VPT; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) aw[j][i] = ab[j][i] = 0.f;
+    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.M; r0 += (int64_t)gridDim.x * RPB) {
+        const int64_t row = r0 + grp;
+        const bool ok = row < a.M;
+        const T* xr = (const T*)a.x + (ok ? row : 0) * a.ldx;
+        const T* dr = (const T*)a.dy + (ok ? row : 0) * a.lddy;
+        const float mean = ok ? a.mean[row] : 0.f, rstd = ok ? a.rstd[row] : 0.f;
+        // a row's x and dy, dy without what dropout and ReLU take away: du = ds dc.  (AGAIN: too many for the
+        // registers beside the sums; each phase reads them, the second with the first's bits)
+        Chunk<T> xc[AGAIN ? 1 : VPT], dc[AGAIN ? 1 : VPT];
+        uint32_t bits[VPT];
+        auto read = [&](int j) {
+            const int col = (j * TPR + lane) * 8;
+            Chunk<T>&x = xc[AGAIN ? 0 : j], &d = dc[AGAIN ? 0 : j];
+            x = ld_row<EVEN>(xr, col, N);
+            d = ld_row<EVEN>(dr, col, N);
+            if ((EVEN && col >= N) || !ok) d = Chunk<T>{};  // adds nothing
+        };
+        if constexpr (!AGAIN) {
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) read(j);
+        }
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            if constexpr (AGAIN) read(j);
+            const int c = j * TPR + lane, col = c * 8, n = N - col;
+            Chunk<T>&x = xc[AGAIN ? 0 : j], &dd = dc[AGAIN ? 0 : j];
+            float w[8], b[8];
+            if constexpr (HOLD) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[i] = hw[HOLD ? j : 0][i];
+            } else {  // (a chunk behind the row's end multiplies zeros)
+                lds_get8(lds_anew(lw), slots, c < slots ? c : 0, w);
+            }
+            if (MASK) {
+                bool on[8] = {true, true, true, true, true, true, true, true};
+                if (a.drop.thr) keep8(a.drop, row, c, on);
+                if (a.relu) {
+                    ldw<T>(a.b, a.wf32, col, n, 0.f, b);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) on[i] = on[i] && ln_u(x.get(i), mean, rstd, w[i], b[i]) > 0.f;
+                }
+                dd.keep(on);
+                if constexpr (AGAIN) {
+                    bits[j] = 0;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) bits[j] |= on[i] ? 1u << i : 0u;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float xh = (x.get(i) - mean) * rstd;
+                const float d = MASK ? dd.get(i) * ds : dd.get(i);
+                const float dxh = d * xh;
+                aw[j][i] += dxh;
+                ab[j][i] += d;
+                s1 = __builtin_fmaf(d, w[i], s1);
+                s2 = __builtin_fmaf(dxh, w[i], s2);
+            }
+            // chunk by chunk, each sum taken here: the products of all chunks at once, kept for sums further
+            // down, would not fit the registers
+            if constexpr (VPT > 1) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(aw[j][i]), "+v"(ab[j][i]));
+                asm volatile("" : "+v"(s1), "+v"(s2));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        if (a.y) {
+            if constexpr (VPT > 1 && !AGAIN) {
+#pragma unroll
+                for (int j = 0; j < VPT; ++j) {
+                    xc[j].anew();
+                    dc[j].anew();
+                }
+            }
+            const float c1 = row_sum<TPR>(s1, red[0]) * inv, c2 = row_sum<TPR>(s2, red[1]) * inv;
+            if (ok) {
+                T* yr = (T*)a.y + row * a.ldy;
+#pragma unroll
+                for (int j = 0; j < VPT; ++j) {
+                    const int col = (j * TPR + lane) * 8, n = N - col;
+                    if (n <= 0) continue;
+                    if constexpr (AGAIN) {
+                        read(j);
+                        bool on[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) on[i] = (bits[j] >> i) & 1;
+                        if (MASK) dc[0].keep(on);
+                    }
+                    const Chunk<T>&x = xc[AGAIN ? 0 : j], &dd = dc[AGAIN ? 0 : j];
+                    float w[8];
+                    if constexpr (HOLD) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) w[i] = hw[HOLD ? j : 0][i];
+                    } else {
+                        lds_get8(lds_anew(lw), slots, j * TPR + lane, w);
+                    }
+                    Chunk<T> o;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float xh = (x.get(i) - mean) * rstd;
+                        const float d = MASK ? dd.get(i) * ds : dd.get(i);
+                        o.set(i, rstd * (__builtin_fmaf(d, w[i], -c1) - xh * c2));
+                    }
+                    if constexpr (EVEN) o.store(yr + col);
+                    else st8(yr + col, n, o);
+                    if constexpr (VPT > 1) __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        }
+        if constexpr (TPR > 64) __syncthreads();
+    }
+    if (!a.part && !a.dw && !a.db) return;
+    // a column's sum: into the partials, or (one workgroup) rounded into the gradients
+    auto put = [&](int h, int c, float v) {
+        if (a.part) {
+            a.part[((int64_t)blockIdx.x * 2 + h) * a.Np + c] = v;
+        } else if (c < N) {
+            void* o = h ? a.db : a.dw;
+            if (!o) return;
+            if (a.wf32) ((float*)o)[c] = v;
+            else ((T*)o)[c] = (T)v;
+        }
+    };
+    if constexpr (RPB == 1) {
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int col = (j * TPR + lane) * 8;
+            if (col < N) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {  // (Np is a multiple of 8)
+                    put(0, col + i, aw[j][i]);
+                    put(1, col + i, ab[j][i]);
+                }
+            }
+        }
+    } else {
+        __shared__ float sh[RPB][TPR * VPT * 8];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < VPT; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sh[grp][(j * TPR + lane) * 8 + i] = h ? ab[j][i] : aw[j][i];
+            __syncthreads();
+            for (int c = threadIdx.x; c < TPR * VPT * 8; c += BLK) {
+                float t = 0.f;
+#pragma unroll 8
+                for (int g = 0; g < RPB; ++g) t += sh[g][c];
+                if (c < a.Np) put(h, c, t);
+            }
+        }
+    }
+}
+
+// dw / db: the G partial rows of a column summed in a fixed order (workgroup: 32 columns x 32 row
+// groups, a group's loads four at a time)
+template <class W>
+__global__ __launch_bounds__(1024) void k_ln_wred(int N, int64_t Np, int G, const float* __restrict__ part, W* __restrict__ dw,
+                                                  W* __restrict__ db) {
+    __shared__ float sh[32][33];
+    const int lane = threadIdx.x & 31, g0 = threadIdx.x >> 5;
+    const int64_t col = (int64_t)blockIdx.x * 32 + lane;  // of [2][Np]
+    const int64_t cc = col < 2 * Np ? col : 0;
+    float t = 0.f;
+    for (int g = g0; g < G; g += 128) {
+        float v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = part[(int64_t)min(g + 32 * k, G - 1) * 2 * Np + cc];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) t += g + 32 * k < G ? v[k] : 0.f;
+    }
+    sh[g0][lane] = t;
+    __syncthreads();
+    if (threadIdx.x < 32 && col < 2 * Np) {
+        t = 0.f;
+#pragma unroll
+        for (int g = 0; g < 32; ++g) t += sh[g][lane];
+        const bool second = col >= Np;
+        const int64_t c = second ? col - Np : col;
+        W* o = second ? db : dw;
+        if (o && c < N) o[c] = (W)t;
+    }
+}
+
+// Rows too long for the registers (N > 32,768): each sweep reads the row again
+static constexpr int LONG_N = 32768;
+template <class T> __global__ __launch_bounds__(1024) void k_ln_fwd_long(NormP a) {
+    __shared__ float red[2][16];
+    const int N = a.N;
+    const float inv = 1.f / (float)N;
+    drop_state(a.drop);
+    for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
+        const T* xr = (const T*)a.x + row * a.ldx;
+        float s = 0.f;
+        for (int64_t col = threadIdx.x * 8; col < N; col += 8192) {
+            const Chunk<T> c = ld8(xr + col, (int)(N - col));
+            float t = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t += c.get(i);
+            s += t;
+        }
+        const float mean = row_sum<1024>(s, red[0]) * inv;
+        float q = 0.f;
+        for (int64_t col = threadIdx.x * 8; col < N; col += 8192) {
+            const int n = (int)(N - col);
+            const Chunk<T> c = ld8(xr + col, n);
+            float t = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float d = c.get(i) - mean;
+                t += i < n ? d * d : 0.f;
+            }
+            q += t;
+        }
+        const float rstd = 1.f / sqrtf(row_sum<1024>(q, red[1]) * inv + a.eps);
+        T* yr = (T*)a.y + row * a.ldy;
+        for (int64_t col = threadIdx.x * 8; col < N; col += 8192) {
+            const int n = (int)(N - col);
+            const Chunk<T> c = ld8(xr + col, n);
+            float w[8], b[8];
+            bool kept[8];
+            ldw<T>(a.w, a.wf32, (int)col, n, 1.f, w);
+            ldw<T>(a.b, a.wf32, (int)col, n, 0.f, b);
+            if (a.drop.thr) keep8(a.drop, row, (int)(col >> 3), kept);
+            Chunk<T> yc;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float u = ln_u(c.get(i), mean, rstd, w[i], b[i]);
+                if (a.relu) u = u > 0.f || u != u ? u : 0.f;
+                if (a.drop.thr) u = kept[i] ? u * a.drop.s : 0.f;
+                yc.set(i, u);
+            }
+            st8(yr + col, n, yc);
+        }
+        if (threadIdx.x == 0) {
+            if (a.mean) a.mean[row] = mean;
+            if (a.rstd) a.rstd[row] = rstd;
+        }
+        __syncthreads();
+    }
+}
+// one chunk's du and xh
+template <class T>
+MMVAE_DEV void ln_du(const NormP& a, int64_t row, int64_t col, float mean, float rstd, float w[8], float du[8], float xh[8]) {
+    const int n = (int)(a.N - col);
+    const Chunk<T> xc = ld8((const T*)a.x + row * a.ldx + col, n), dc = ld8((const T*)a.dy + row * a.lddy + col, n);
+    float b[8];
+    bool kept[8];
+    ldw<T>(a.w, a.wf32, (int)col, n, 1.f, w);
+    if (a.relu) ldw<T>(a.b, a.wf32, (int)col, n, 0.f, b);
+    if (a.drop.thr) keep8(a.drop, row, (int)(col >> 3), kept);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        xh[i] = i < n ? (xc.get(i) - mean) * rstd : 0.f;
+        float d = dc.get(i);
+        if (a.drop.thr) d = kept[i] ? d * a.drop.s : 0.f;
+        if (a.relu) d = ln_u(xc.get(i), mean, rstd, w[i], b[i]) > 0.f ? d : 0.f;
+        du[i] = i < n ? d : 0.f;
+    }
+}
+template <class T> __global__ __launch_bounds__(1024) void k_ln_bwd_long(NormP a) {
+    __shared__ float red[2][16];
+    const float inv = 1.f / (float)a.N;
+    drop_state(a.drop);
+    for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        float s1 = 0.f, s2 = 0.f, w[8], du[8], xh[8];
+        for (int64_t col = threadIdx.x * 8; col < a.N; col += 8192) {
+            ln_du<T>(a, row, col, mean, rstd, w, du, xh);
+            float t1 = 0.f, t2 = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                t1 = __builtin_fmaf(du[i], w[i], t1);
+                t2 = __builtin_fmaf(du[i] * xh[i], w[i], t2);
+            }
+            s1 += t1;
+            s2 += t2;
+        }
+        const float c1 = row_sum<1024>(s1, red[0]) * inv, c2 = row_sum<1024>(s2, red[1]) * inv;
+        T* yr = (T*)a.y + row * a.ldy;
+        for (int64_t col = threadIdx.x * 8; col < a.N; col += 8192) {
+            ln_du<T>(a, row, col, mean, rstd, w, du, xh);
+            Chunk<T> o;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o.set(i, rstd * (__builtin_fmaf(du[i], w[i], -c1) - xh[i] * c2));
+            st8(yr + col, (int)(a.N - col), o);
+        }
+        __syncthreads();
+    }
+}
+// their weight gradients: thread = a chunk of columns, workgroup row y = a stripe of rows
+template <class T> __global__ __launch_bounds__(256) void k_ln_cols(NormP a) {
+    const int64_t col = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+    if (col >= a.N) return;
+    drop_state(a.drop);
+    float aw[8] = {}, ab[8] = {}, w[8], du[8], xh[8];
+    for (int64_t row = blockIdx.y; row < a.M; row += gridDim.y) {
+        ln_du<T>(a, row, col, a.mean[row], a.rstd[row], w, du, xh);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            aw[i] += du[i] * xh[i];
+            ab[i] += du[i];
+        }
+    }
+    float* pw = a.part + (int64_t)blockIdx.y * 2 * a.Np;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        pw[col + i] = aw[i];
+        pw[a.Np + col + i] = ab[i];
+    }
+}
+
+// =======================================================================================
+// Host side
+// =======================================================================================
+// the row layout by width: threads per row, chunks per thread, threads per workgroup.  Up to 64 lanes a
+// row stays inside a wave and needs no barrier.
+template <class F> inline hipError_t by_width(int N, F&& f) {
+    const int nc = (N + 7) / 8;
+    if (nc <= 8) return f(I<8>{}, I<1>{}, I<256>{});
+    if (nc <= 16) return f(I<16>{}, I<1>{}, I<256>{});
+    if (nc <= 32) return f(I<32>{}, I<1>{}, I<256>{});
+    if (nc <= 64) return f(I<64>{}, I<1>{}, I<256>{});
+    if (nc <= 128) return f(I<64>{}, I<2>{}, I<256>{});
+    if (nc <= 256) return f(I<256>{}, I<1>{}, I<256>{});
+    if (nc <= 512) return f(I<256>{}, I<2>{}, I<256>{});
+    if (nc <= 1024) return f(I<512>{}, I<2>{}, I<512>{});
+    if (nc <= 2048) return f(I<1024>{}, I<2>{}, I<1024>{});
+    if (nc <= 3072) return f(I<1024>{}, I<3>{}, I<1024>{});
+    return f(I<1024>{}, I<4>{}, I<1024>{});
+}
+// a backward of few rows in one workgroup of 1024, which writes dw and db itself: rows it may have
+constexpr int ONE_ROUNDS = 2;
+inline bool norm_one(int64_t M, int64_t N) {
+    const int nc = (int)((std::min<int64_t>(N, LONG_N) + 7) / 8);
+    int tpr = 8;
+    while (tpr < 64 && tpr < nc) tpr *= 2;
+    return N <= 1024 ? M <= ONE_ROUNDS * (1024 / tpr) : N <= LONG_N && M <= 1;
+}
+template <class F> inline hipError_t by_width_one(int N, F&& f) {
+    const int nc = (N + 7) / 8;
+    if (nc <= 8) return f(I<8>{}, I<1>{}, I<1024>{});
+    if (nc <= 16) return f(I<16>{}, I<1>{}, I<1024>{});
+    if (nc <= 32) return f(I<32>{}, I<1>{}, I<1024>{});
+    if (nc <= 64) return f(I<64>{}, I<1>{}, I<1024>{});
+    if (nc <= 128) return f(I<64>{}, I<2>{}, I<1024>{});
+    return by_width(N, f);
+}
+inline NormP norm_p(const mmvae_norm_args& a) {
+    NormP p;
+    std::memset(&p, 0, sizeof(p));
+    p.M = a.M;
+    p.N = (int)a.N;
+    p.x = a.x;
+    p.ldx = a.ldx;
+    p.w = a.w;
+    p.b = a.b;
+    p.mean = a.mean;
+    p.rstd = a.rstd;
+    p.eps = a.eps;
+    p.relu = a.relu;
+    p.wf32 = a.wtype == MMVAE_T_F32;
+    p.Np = (a.N + 7) / 8 * 8;
+    p.drop = drop_key(a.p, a.seed, a.step, a.row_offset, a.state);
+    return p;
+}
+inline int norm_rpb(int64_t N) {  // rows a workgroup holds at once
+    int r = 1;
+    (void)by_width((int)std::min<int64_t>(N, LONG_N), [&](auto t, auto, auto b) {
+        r = b.value / t.value;
+        return hipSuccess;
+    });
+    return r;
+}
+// workgroups of the backward = rows of partial weight sums
+inline int64_t norm_parts(int64_t M, int64_t N) {
+    if (norm_one(M, N)) return 1;
+    if (N > LONG_N) return std::min<int64_t>(M, 32);
+    const int64_t need = (M + norm_rpb(N) - 1) / norm_rpb(N);
+    return std::min<int64_t>(need, N > 8192 ? 256 : 512);
+}
+inline int64_t norm_ws_bytes(int64_t M, int64_t N) {
+    if (norm_one(M, N)) return 0;
+    return norm_parts(std::max<int64_t>(M, 1), N) * 2 * ((N + 7) / 8 * 8) * (int64_t)sizeof(float);
+}
+
+// with a ReLU or dropout; N a multiple of the chunk
+template <class F> inline hipError_t by_flags(const NormP& p, F&& f) {
+    const bool m = p.relu || p.drop.thr, e = p.N % 8 == 0;
+    if (m) return e ? f(std::true_type{}, std::true_type{}) : f(std::true_type{}, std::false_type{});
+    return e ? f(std::false_type{}, std::true_type{}) : f(std::false_type{}, std::false_type{});
+}
+
+template <class T> hipError_t norm_fwd_t(const mmvae_norm_args& a, hipStream_t st) {
+    NormP p = norm_p(a);
+    p.y = a.y;
+    p.ldy = a.ldy;
+    if (a.N > LONG_N) return launch(k_ln_fwd_long<T>, dim3((unsigned)std::min<int64_t>(a.M, 512)), dim3(1024), st, p);
+    return by_width(p.N, [&](auto t, auto v, auto b) -> hipError_t {
+        constexpr int RPB = b.value / t.value;
+        const int64_t g = std::min<int64_t>((a.M + RPB - 1) / RPB, 256 * (2048 / b.value));
+        size_t lds = 0;
+        if (LnHold<b.value>::LDS) {
+            p.b_lds = 2 * p.Np * 4 <= LN_LDS - 256;  // (beside the waves' sums)
+            lds = (p.b_lds ? 2 : 1) * (size_t)p.Np * 4;
+        }
+        return by_flags(p, [&](auto m, auto e) {
+            return launch_lds(lds, k_ln_fwd<T, t.value, v.value, b.value, m.value, e.value>, dim3((unsigned)g), dim3(b.value), st, p);
+        });
+    });
+}
+
+template <class T> hipError_t norm_bwd_t(const mmvae_norm_args& a, hipStream_t st) {
+    NormP p = norm_p(a);
+    p.dy = a.dy;
+    p.lddy = a.lddy;
+    p.y = a.dx;
+    p.ldy = a.lddx;
+    const bool wg = a.dw || a.db, one = norm_one(a.M, a.N) && a.M > 0;
+    p.part = wg && !one ? (float*)a.ws : nullptr;
+    p.dw = a.dw;
+    p.db = a.db;
+    const int64_t G = norm_parts(a.M, a.N);
+    if (a.M > 0 && (a.dx || wg)) {
+        if (a.N > LONG_N) {
+            if (wg)  // (first: dx may overwrite dy or x)
+                OPCHK(launch(k_ln_cols<T>, dim3((unsigned)((p.Np / 8 + 255) / 256), (unsigned)G), dim3(256), st, p));
+            if (a.dx) OPCHK(launch(k_ln_bwd_long<T>, dim3((unsigned)std::min<int64_t>(a.M, 512)), dim3(1024), st, p));
+        } else {
+            auto go = [&](auto t, auto v, auto b) -> hipError_t {
+                const size_t lds = LnHold<b.value>::LDS && t.value > 64 ? (size_t)p.Np * 4 : 0;
+                return by_flags(p, [&](auto m, auto e) {
+                    return launch_lds(lds, k_ln_bwd<T, t.value, v.value, b.value, m.value, e.value>, dim3((unsigned)G), dim3(b.value), st, p);
+                });
+            };
+            OPCHK(one ? by_width_one(p.N, go) : by_width(p.N, go));
+        }
+    }
+    if (!wg || one) return hipSuccess;
+    const dim3 grid((unsigned)((2 * p.Np + 31) / 32));
+    const int parts = (int)(a.M > 0 ? G : 0);
+    if (p.wf32)
+        return launch(k_ln_wred<float>, grid, dim3(1024), st, p.N, p.Np, parts, (const float*)a.ws, (float*)a.dw, (float*)a.db);
+    return launch(k_ln_wred<T>, grid, dim3(1024), st, p.N, p.Np, parts, (const float*)a.ws, (T*)a.dw, (T*)a.db);
+}
+
+}  // namespace mmvae

@@ -1,513 +1,15 @@
 // Layer operators on device tensors (mmvae_layer_norm_*, mmvae_dropout, mmvae_embedding_*): the
 // normalised, dropped-out, label-conditioned layer chain of the wide path (wide.hip), and the
-// same for callers with tensors of their own.
+// same for callers with tensors of their own.  The norm's kernels: norm.hpp.
 //
 // Every kernel moves 8 consecutive elements per lane ("a chunk": 16 B of bf16 / f16, 32 B of f32),
 // which is also what one Philox call masks.  Chunks are loaded at the elements' own alignment, so
-// odd widths and row strides take the same path; only a row's last, partial chunk goes element by
-// element.  Sums, statistics and accumulators are f32; a value is rounded to its type once, when
-// it is stored.  Every reduction has a fixed order, so equal calls give equal bits.
-#include <algorithm>
-#include <cmath>
-#include <cstring>
-#include <tuple>
-#include <type_traits>
-
-#include "common.hpp"
-#include "engine.hpp"
-#include "ops.hpp"
+// odd widths and row strides take the same path; a row's last, partial chunk goes in pieces.
+// Sums, statistics and accumulators are f32; a value is rounded to its type once, when it is
+// stored.  Every reduction has a fixed order, so equal calls give equal bits.
+#include "ops_dev.hpp"
 
 namespace mmvae {
-
-// =======================================================================================
-// Chunks: 8 consecutive elements
-// =======================================================================================
-typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
-typedef __bf16 bf16x8u __attribute__((ext_vector_type(8), aligned(2)));
-typedef _Float16 f16x8u __attribute__((ext_vector_type(8), aligned(2)));
-
-template <class T> struct Chunk;
-template <> struct Chunk<float> {
-    f32x4u a, b;
-    MMVAE_DEV float get(int i) const { return i < 4 ? a[i & 3] : b[i & 3]; }
-    MMVAE_DEV void set(int i, float v) {
-        if (i < 4) a[i & 3] = v;
-        else b[i & 3] = v;
-    }
-    static MMVAE_DEV Chunk load(const float* p) {
-        return Chunk{*reinterpret_cast<const f32x4u*>(p), *reinterpret_cast<const f32x4u*>(p + 4)};
-    }
-    MMVAE_DEV void store(float* p) const {
-        *reinterpret_cast<f32x4u*>(p) = a;
-        *reinterpret_cast<f32x4u*>(p + 4) = b;
-    }
-};
-template <class T, class V> struct Chunk16 {
-    V v;
-    MMVAE_DEV float get(int i) const { return (float)v[i]; }
-    MMVAE_DEV void set(int i, float x) { v[i] = (T)x; }  // to nearest even
-};
-template <> struct Chunk<__bf16> : Chunk16<__bf16, bf16x8u> {
-    static MMVAE_DEV Chunk load(const __bf16* p) {
-        Chunk c;
-        c.v = *reinterpret_cast<const bf16x8u*>(p);
-        return c;
-    }
-    MMVAE_DEV void store(__bf16* p) const { *reinterpret_cast<bf16x8u*>(p) = v; }
-};
-template <> struct Chunk<_Float16> : Chunk16<_Float16, f16x8u> {
-    static MMVAE_DEV Chunk load(const _Float16* p) {
-        Chunk c;
-        c.v = *reinterpret_cast<const f16x8u*>(p);
-        return c;
-    }
-    MMVAE_DEV void store(_Float16* p) const { *reinterpret_cast<f16x8u*>(p) = v; }
-};
-
-// the n valid elements of a chunk (n <= 0: none), zeros behind them
-template <class T> MMVAE_DEV Chunk<T> ld8(const T* p, int n) {
-    if (n >= 8) return Chunk<T>::load(p);
-    Chunk<T> c;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c.set(i, i < n ? (float)p[i] : 0.f);
-    return c;
-}
-template <class T> MMVAE_DEV void st8(T* p, int n, const Chunk<T>& c) {
-    if (n >= 8) {
-        c.store(p);
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (i < n) p[i] = (T)c.get(i);
-}
-// 8 weights of type T or f32 (w null: `none`)
-template <class T> MMVAE_DEV void ldw(const void* w, bool f32, int col, int n, float none, float v[8]) {
-    if (!w) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = none;
-    } else if (f32) {
-        const Chunk<float> c = ld8((const float*)w + col, n);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c.get(i);
-    } else {
-        const Chunk<T> c = ld8((const T*)w + col, n);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c.get(i);
-    }
-}
-
-// =======================================================================================
-// Sums over the TPR lanes of a row (every lane gets the sum), in registers: DPP within 16 lanes,
-// then the two lane swaps
-// =======================================================================================
-template <int CTRL> MMVAE_DEV float dpp_add(float v) {
-    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
-}
-template <int TPR> MMVAE_DEV float lanes_sum(float v) {
-    v = dpp_add<0xB1>(v);                        // quad_perm [1, 0, 3, 2]
-    v = dpp_add<0x4E>(v);                        // quad_perm [2, 3, 0, 1]
-    v = dpp_add<0x141>(v);                       // row_half_mirror: the other quad of 8 lanes
-    if constexpr (TPR >= 16) v = dpp_add<0x140>(v);  // row_mirror: the other 8 of 16 lanes
-    if constexpr (TPR >= 32) {
-        const unsigned u = __builtin_bit_cast(unsigned, v);
-        const auto s = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-        v = __builtin_bit_cast(float, (unsigned)s[0]) + __builtin_bit_cast(float, (unsigned)s[1]);
-    }
-    if constexpr (TPR >= 64) {
-        const unsigned u = __builtin_bit_cast(unsigned, v);
-        const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-        v = __builtin_bit_cast(float, (unsigned)s[0]) + __builtin_bit_cast(float, (unsigned)s[1]);
-    }
-    return v;
-}
-// the same over a row's TPR > 64 threads (one row per workgroup): the waves' sums through `red`
-template <int TPR> MMVAE_DEV float row_sum(float v, float* red) {
-    v = lanes_sum<(TPR < 64 ? TPR : 64)>(v);
-    if constexpr (TPR > 64) {
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = 0.f;
-#pragma unroll
-        for (int w = 0; w < TPR / 64; ++w) v += red[w];
-    }
-    return v;
-}
-
-// =======================================================================================
-// Dropout factors.  16 random bits per element: half (col % 8) of the four words of
-// Philox4x32-10 at the counter (col / 8, row, step, step >> 32 ^ row >> 32), keyed by the seed;
-// kept iff they are >= thr = round(65536 p), so P(kept) = 1 - thr / 65536 exactly and the factor
-// 65536 / (65536 - thr) leaves the mean unchanged.  The row is global (row_offset + r), so the
-// shards of a data-parallel batch drop what the whole batch would; the mask is never stored: the
-// backward recomputes it.  Cost: 20 32 x 32-bit products per 8 elements.
-// =======================================================================================
-struct DropKey {
-    uint32_t thr;  // 0: no dropout
-    float s;
-    uint32_t k0, k1;
-    int64_t step, row0;
-    const int64_t* state;
-};
-MMVAE_DEV void drop_state(DropKey& k) {
-    if (k.state) {
-        k.step += k.state[0];
-        k.row0 += k.state[1];
-    }
-}
-MMVAE_DEV void drop8(const DropKey& k, int64_t row, int chunk, float f[8]) {
-    const uint64_t r = (uint64_t)(k.row0 + row);
-    uint32_t c[4] = {(uint32_t)chunk, (uint32_t)r, (uint32_t)k.step, (uint32_t)((uint64_t)k.step >> 32) ^ (uint32_t)(r >> 32)};
-    philox4x32_10(c, k.k0, k.k1);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint32_t h = (i & 1) ? c[i >> 1] >> 16 : c[i >> 1] & 0xffffu;
-        f[i] = h >= k.thr ? k.s : 0.f;
-    }
-}
-
-// A dropped element is 0 whatever it was (an infinity or NaN times the factor 0 would be NaN)
-MMVAE_DEV float drop_mul(float v, float f) { return f != 0.f ? v * f : 0.f; }
-
-// =======================================================================================
-// Layer norm over rows of N: y = drop(act(xh w + b)), xh = (x - mean) rstd
-// TPR threads hold a row (VPT chunks each) in registers: x is read once, the variance is the
-// mean square of the differences from the mean.
-// =======================================================================================
-struct NormP {
-    int64_t M;
-    int N;
-    const void *x, *w, *b, *dy;
-    int64_t ldx, lddy, ldy;  // ldy: of y, or of dx
-    void* y;                 // y, or dx
-    float *mean, *rstd;
-    float* part;             // backward: the workgroups' sums [grid][2][Np] (null: no weight gradients)
-    int64_t Np;
-    float eps;
-    int relu;
-    bool wf32;
-    DropKey drop;
-};
-
-template <class T, int TPR, int VPT, int BLK>
-__global__ __launch_bounds__(BLK) void k_ln_fwd(NormP a) {
-    constexpr int RPB = BLK / TPR;
-    __shared__ float red[2][BLK / 64];
-    const int lane = threadIdx.x % TPR, grp = threadIdx.x / TPR;
-    const int N = a.N;
-    const float inv = 1.f / (float)N;
-    drop_state(a.drop);
-    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.M; r0 += (int64_t)gridDim.x * RPB) {
-        const int64_t row = r0 + grp;
-        const bool ok = row < a.M;
-        const T* xr = (const T*)a.x + (ok ? row : 0) * a.ldx;
-        Chunk<T> xc[VPT];
-        float s = 0.f;
-#pragma unroll
-        for (int j = 0; j < VPT; ++j) {
-            const int col = (j * TPR + lane) * 8;
-            xc[j] = ld8(xr + col, ok ? N - col : 0);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s += xc[j].get(i);
-        }
-        const float mean = row_sum<TPR>(s, red[0]) * inv;
-        float q = 0.f;
-#pragma unroll
-        for (int j = 0; j < VPT; ++j) {
-            const int n = N - (j * TPR + lane) * 8;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float d = xc[j].get(i) - mean;
-                q += i < n ? d * d : 0.f;
-            }
-        }
-        const float rstd = 1.f / sqrtf(row_sum<TPR>(q, red[1]) * inv + a.eps);
-        if (ok) {
-            T* yr = (T*)a.y + row * a.ldy;
-#pragma unroll
-            for (int j = 0; j < VPT; ++j) {
-                const int c = j * TPR + lane, col = c * 8, n = N - col;
-                if (n <= 0) continue;
-                float w[8], b[8], f[8];
-                ldw<T>(a.w, a.wf32, col, n, 1.f, w);
-                ldw<T>(a.b, a.wf32, col, n, 0.f, b);
-                if (a.drop.thr) drop8(a.drop, row, c, f);
-                Chunk<T> yc;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    float u = __builtin_fmaf((xc[j].get(i) - mean) * rstd, w[i], b[i]);
-                    if (a.relu) u = u > 0.f || u != u ? u : 0.f;  // (a NaN stays one)
-                    if (a.drop.thr) u = drop_mul(u, f[i]);
-                    yc.set(i, u);
-                }
-                st8(yr + col, n, yc);
-            }
-            if (lane == 0) {
-                if (a.mean) a.mean[row] = mean;
-                if (a.rstd) a.rstd[row] = rstd;
-            }
-        }
-        if constexpr (TPR > 64) __syncthreads();  // the next row's sums reuse `red`
-    }
-}
-
-// backward: du = dy m [u > 0], g = du w, dx = rstd (g - mean(g) - xh mean(g xh)); the workgroup's
-// sums of du xh and du over its rows -> part (fixed order: a thread's rows, then the row groups)
-template <class T, int TPR, int VPT, int BLK>
-__global__ __launch_bounds__(BLK) void k_ln_bwd(NormP a) {
-    constexpr int RPB = BLK / TPR;
-    __shared__ float red[2][BLK / 64];
-    const int lane = threadIdx.x % TPR, grp = threadIdx.x / TPR;
-    const int N = a.N;
-    const float inv = 1.f / (float)N, ds = a.drop.thr ? a.drop.s : 1.f;
-    drop_state(a.drop);
-    float aw[VPT][8], ab[VPT][8];
-#pragma unroll
-    for (int j = 0; j < VPT; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) aw[j][i] = ab[j][i] = 0.f;
-    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.M; r0 += (int64_t)gridDim.x * RPB) {
-        const int64_t row = r0 + grp;
-        const bool ok = row < a.M;
-        const T* xr = (const T*)a.x + (ok ? row : 0) * a.ldx;
-        const T* dr = (const T*)a.dy + (ok ? row : 0) * a.lddy;
-        const float mean = a.mean[ok ? row : 0], rstd = a.rstd[ok ? row : 0];
-        Chunk<T> xc[VPT], dc[VPT];
-#pragma unroll
-        for (int j = 0; j < VPT; ++j) {
-            const int col = (j * TPR + lane) * 8, n = ok ? N - col : 0;
-            xc[j] = ld8(xr + col, n);
-            dc[j] = ld8(dr + col, n);
-        }
-        // du of an element = bit ? dy s : 0 (bit: kept, past the ReLU, inside the row)
-        float s1 = 0.f, s2 = 0.f;
-        uint32_t bits[VPT];
-#pragma unroll
-        for (int j = 0; j < VPT; ++j) {
-            const int c = j * TPR + lane, col = c * 8, n = ok ? N - col : 0;
-            bits[j] = n >= 8 ? 255u : n > 0 ? (1u << n) - 1u : 0u;
-            float w[8], b[8], f[8];
-            ldw<T>(a.w, a.wf32, col, n, 1.f, w);
-            if (a.relu) ldw<T>(a.b, a.wf32, col, n, 0.f, b);
-            if (a.drop.thr) drop8(a.drop, row, c, f);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float xh = (xc[j].get(i) - mean) * rstd;
-                if (a.drop.thr) bits[j] &= f[i] != 0.f ? ~0u : ~(1u << i);
-                if (a.relu) bits[j] &= __builtin_fmaf(xh, w[i], b[i]) > 0.f ? ~0u : ~(1u << i);
-                const float d = (bits[j] >> i) & 1 ? dc[j].get(i) * ds : 0.f;
-                const float dxh = i < n ? d * xh : 0.f;
-                aw[j][i] += dxh;
-                ab[j][i] += d;
-                s1 = __builtin_fmaf(d, w[i], s1);
-                s2 = __builtin_fmaf(dxh, w[i], s2);
-            }
-        }
-        if (a.y) {
-            const float c1 = row_sum<TPR>(s1, red[0]) * inv, c2 = row_sum<TPR>(s2, red[1]) * inv;
-            if (ok) {
-                T* yr = (T*)a.y + row * a.ldy;
-#pragma unroll
-                for (int j = 0; j < VPT; ++j) {
-                    const int col = (j * TPR + lane) * 8, n = N - col;
-                    if (n <= 0) continue;
-                    float w[8];
-                    ldw<T>(a.w, a.wf32, col, n, 1.f, w);
-                    Chunk<T> o;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float xh = (xc[j].get(i) - mean) * rstd;
-                        const float d = (bits[j] >> i) & 1 ? dc[j].get(i) * ds : 0.f;
-                        o.set(i, rstd * (__builtin_fmaf(d, w[i], -c1) - xh * c2));
-                    }
-                    st8(yr + col, n, o);
-                }
-            }
-        }
-        if constexpr (TPR > 64) __syncthreads();
-    }
-    if (!a.part) return;
-    float* pw = a.part + (int64_t)blockIdx.x * 2 * a.Np;
-    if constexpr (RPB == 1) {
-#pragma unroll
-        for (int j = 0; j < VPT; ++j) {
-            const int col = (j * TPR + lane) * 8;
-            if (col < N) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {  // (Np is a multiple of 8)
-                    pw[col + i] = aw[j][i];
-                    pw[a.Np + col + i] = ab[j][i];
-                }
-            }
-        }
-    } else {
-        __shared__ float sh[RPB][TPR * VPT * 8];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < VPT; ++j)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sh[grp][(j * TPR + lane) * 8 + i] = h ? ab[j][i] : aw[j][i];
-            __syncthreads();
-            for (int c = threadIdx.x; c < TPR * VPT * 8; c += BLK) {
-                float t = 0.f;
-#pragma unroll
-                for (int g = 0; g < RPB; ++g) t += sh[g][c];
-                if (c < a.Np) pw[h * a.Np + c] = t;
-            }
-        }
-    }
-}
-
-// dw / db: the G partial rows of a column summed in a fixed order (16 row groups of 64 columns)
-template <class W>
-__global__ __launch_bounds__(1024) void k_ln_wred(int N, int64_t Np, int G, const float* __restrict__ part, W* __restrict__ dw,
-                                                  W* __restrict__ db) {
-    __shared__ float sh[16][64];
-    const int lane = threadIdx.x & 63, g0 = threadIdx.x >> 6;
-    const int64_t col = (int64_t)blockIdx.x * 64 + lane;  // of [2][Np]
-    float t = 0.f;
-    if (col < 2 * Np)
-        for (int g = g0; g < G; g += 16) t += part[(int64_t)g * 2 * Np + col];
-    sh[g0][lane] = t;
-    __syncthreads();
-    if (g0 == 0 && col < 2 * Np) {
-        t = 0.f;
-#pragma unroll
-        for (int g = 0; g < 16; ++g) t += sh[g][lane];
-        const bool second = col >= Np;
-        const int64_t c = second ? col - Np : col;
-        W* o = second ? db : dw;
-        if (o && c < N) o[c] = (W)t;
-    }
-}
-
-// Rows too long for the registers (N > 32,768): each sweep reads the row again
-static constexpr int LONG_N = 32768;
-template <class T> __global__ __launch_bounds__(1024) void k_ln_fwd_long(NormP a) {
-    __shared__ float red[2][16];
-    const int N = a.N;
-    const float inv = 1.f / (float)N;
-    drop_state(a.drop);
-    for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
-        const T* xr = (const T*)a.x + row * a.ldx;
-        float s = 0.f;
-        for (int64_t col = threadIdx.x * 8; col < N; col += 8192) {
-            const Chunk<T> c = ld8(xr + col, (int)(N - col));
-            float t = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) t += c.get(i);
-            s += t;
-        }
-        const float mean = row_sum<1024>(s, red[0]) * inv;
-        float q = 0.f;
-        for (int64_t col = threadIdx.x * 8; col < N; col += 8192) {
-            const int n = (int)(N - col);
-            const Chunk<T> c = ld8(xr + col, n);
-            float t = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float d = c.get(i) - mean;
-                t += i < n ? d * d : 0.f;
-            }
-            q += t;
-        }
-        const float rstd = 1.f / sqrtf(row_sum<1024>(q, red[1]) * inv + a.eps);
-        T* yr = (T*)a.y + row * a.ldy;
-        for (int64_t col = threadIdx.x * 8; col < N; col += 8192) {
-            const int n = (int)(N - col);
-            const Chunk<T> c = ld8(xr + col, n);
-            float w[8], b[8], f[8];
-            ldw<T>(a.w, a.wf32, (int)col, n, 1.f, w);
-            ldw<T>(a.b, a.wf32, (int)col, n, 0.f, b);
-            if (a.drop.thr) drop8(a.drop, row, (int)(col >> 3), f);
-            Chunk<T> yc;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float u = __builtin_fmaf((c.get(i) - mean) * rstd, w[i], b[i]);
-                if (a.relu) u = u > 0.f || u != u ? u : 0.f;
-                if (a.drop.thr) u = drop_mul(u, f[i]);
-                yc.set(i, u);
-            }
-            st8(yr + col, n, yc);
-        }
-        if (threadIdx.x == 0) {
-            if (a.mean) a.mean[row] = mean;
-            if (a.rstd) a.rstd[row] = rstd;
-        }
-        __syncthreads();
-    }
-}
-// one chunk's du and xh
-template <class T>
-MMVAE_DEV void ln_du(const NormP& a, int64_t row, int64_t col, float mean, float rstd, float w[8], float du[8], float xh[8]) {
-    const int n = (int)(a.N - col);
-    const Chunk<T> xc = ld8((const T*)a.x + row * a.ldx + col, n), dc = ld8((const T*)a.dy + row * a.lddy + col, n);
-    float b[8], f[8];
-    ldw<T>(a.w, a.wf32, (int)col, n, 1.f, w);
-    if (a.relu) ldw<T>(a.b, a.wf32, (int)col, n, 0.f, b);
-    if (a.drop.thr) drop8(a.drop, row, (int)(col >> 3), f);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        xh[i] = i < n ? (xc.get(i) - mean) * rstd : 0.f;
-        float d = dc.get(i);
-        if (a.drop.thr) d = drop_mul(d, f[i]);
-        if (a.relu) d = __builtin_fmaf(xh[i], w[i], b[i]) > 0.f ? d : 0.f;
-        du[i] = i < n ? d : 0.f;
-    }
-}
-template <class T> __global__ __launch_bounds__(1024) void k_ln_bwd_long(NormP a) {
-    __shared__ float red[2][16];
-    const float inv = 1.f / (float)a.N;
-    drop_state(a.drop);
-    for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
-        const float mean = a.mean[row], rstd = a.rstd[row];
-        float s1 = 0.f, s2 = 0.f, w[8], du[8], xh[8];
-        for (int64_t col = threadIdx.x * 8; col < a.N; col += 8192) {
-            ln_du<T>(a, row, col, mean, rstd, w, du, xh);
-            float t1 = 0.f, t2 = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                t1 = __builtin_fmaf(du[i], w[i], t1);
-                t2 = __builtin_fmaf(du[i] * xh[i], w[i], t2);
-            }
-            s1 += t1;
-            s2 += t2;
-        }
-        const float c1 = row_sum<1024>(s1, red[0]) * inv, c2 = row_sum<1024>(s2, red[1]) * inv;
-        T* yr = (T*)a.y + row * a.ldy;
-        for (int64_t col = threadIdx.x * 8; col < a.N; col += 8192) {
-            ln_du<T>(a, row, col, mean, rstd, w, du, xh);
-            Chunk<T> o;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) o.set(i, rstd * (__builtin_fmaf(du[i], w[i], -c1) - xh[i] * c2));
-            st8(yr + col, (int)(a.N - col), o);
-        }
-        __syncthreads();
-    }
-}
-// their weight gradients: thread = a chunk of columns, workgroup row y = a stripe of rows
-template <class T> __global__ __launch_bounds__(256) void k_ln_cols(NormP a) {
-    const int64_t col = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
-    if (col >= a.N) return;
-    drop_state(a.drop);
-    float aw[8] = {}, ab[8] = {}, w[8], du[8], xh[8];
-    for (int64_t row = blockIdx.y; row < a.M; row += gridDim.y) {
-        ln_du<T>(a, row, col, a.mean[row], a.rstd[row], w, du, xh);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            aw[i] += du[i] * xh[i];
-            ab[i] += du[i];
-        }
-    }
-    float* pw = a.part + (int64_t)blockIdx.y * 2 * a.Np;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        pw[col + i] = aw[i];
-        pw[a.Np + col + i] = ab[i];
-    }
-}
 
 // =======================================================================================
 // Dropout alone: tpr = 2^s threads walk a row's chunks, 256 / tpr rows per workgroup
@@ -523,10 +25,10 @@ __global__ __launch_bounds__(256) void k_dropout(int64_t M, int64_t N, const T* 
         for (int64_t col = lane * 8; col < N; col += tpr * 8) {
             const int n = (int)(N - col < 8 ? N - col : 8);
             Chunk<T> c = ld8(xr + col, n);
-            float f[8];
-            drop8(k, row, (int)(col >> 3), f);
+            bool kept[8];
+            keep8(k, row, (int)(col >> 3), kept);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) c.set(i, drop_mul(c.get(i), f[i]));
+            for (int i = 0; i < 8; ++i) c.set(i, kept[i] ? c.get(i) * k.s : 0.f);
             st8(yr + col, n, c);
         }
     }
@@ -986,56 +488,6 @@ template <class T, int TPR> __global__ __launch_bounds__(256) void k_emb_join(Em
 // =======================================================================================
 // Host side
 // =======================================================================================
-template <class... P, class... A>
-static hipError_t launch(void (*k)(P...), dim3 grid, dim3 block, hipStream_t st, A&&... args) {
-    // the launch's own error (hipGetLastError could return an earlier call's)
-    std::tuple<P...> v{static_cast<P>(args)...};
-    return std::apply(
-        [&](P&... p) {
-            void* ptr[] = {(void*)&p...};
-            return hipLaunchKernel((const void*)k, grid, block, ptr, 0, st);
-        },
-        v);
-}
-#define OPCHK(x)                            \
-    do {                                    \
-        const hipError_t er_ = (x);         \
-        if (er_ != hipSuccess) return er_;  \
-    } while (0)
-
-static uint32_t drop_thr(double p) { return (uint32_t)std::floor(p * 65536. + 0.5); }
-static DropKey drop_key(double p, uint64_t seed, uint64_t step, uint64_t row_offset, const int64_t* state) {
-    DropKey k;
-    k.thr = drop_thr(p);
-    k.s = k.thr < 65536 ? (float)(65536. / (65536. - k.thr)) : 0.f;
-    k.k0 = (uint32_t)seed;
-    k.k1 = (uint32_t)(seed >> 32);
-    k.step = (int64_t)step;
-    k.row0 = (int64_t)row_offset;
-    k.state = state;
-    return k;
-}
-template <class F> static hipError_t by_type(int dtype, F&& f) {
-    if (dtype == MMVAE_T_F32) return f(float{});
-    if (dtype == MMVAE_T_BF16) return f(__bf16{});
-    return f(_Float16{});
-}
-template <int V> using I = std::integral_constant<int, V>;
-// the row layout by width: threads per row, chunks per thread, threads per workgroup
-template <class F> static hipError_t by_width(int N, F&& f) {
-    const int nc = (N + 7) / 8;
-    if (nc <= 8) return f(I<8>{}, I<1>{}, I<256>{});
-    if (nc <= 16) return f(I<16>{}, I<1>{}, I<256>{});
-    if (nc <= 32) return f(I<32>{}, I<1>{}, I<256>{});
-    if (nc <= 64) return f(I<64>{}, I<1>{}, I<256>{});
-    if (nc <= 128) return f(I<64>{}, I<2>{}, I<256>{});
-    if (nc <= 256) return f(I<256>{}, I<1>{}, I<256>{});
-    if (nc <= 512) return f(I<256>{}, I<2>{}, I<256>{});
-    if (nc <= 1024) return f(I<512>{}, I<2>{}, I<512>{});
-    if (nc <= 2048) return f(I<1024>{}, I<2>{}, I<1024>{});
-    if (nc <= 3072) return f(I<1024>{}, I<3>{}, I<1024>{});
-    return f(I<1024>{}, I<4>{}, I<1024>{});
-}
 // threads per row of the chunk-walking kernels
 static int ltpr_for(int64_t N) {
     const int64_t nc = (N + 7) / 8;
@@ -1044,87 +496,12 @@ static int ltpr_for(int64_t N) {
     return l;
 }
 
-static NormP norm_p(const mmvae_norm_args& a) {
-    NormP p;
-    std::memset(&p, 0, sizeof(p));
-    p.M = a.M;
-    p.N = (int)a.N;
-    p.x = a.x;
-    p.ldx = a.ldx;
-    p.w = a.w;
-    p.b = a.b;
-    p.mean = a.mean;
-    p.rstd = a.rstd;
-    p.eps = a.eps;
-    p.relu = a.relu;
-    p.wf32 = a.wtype == MMVAE_T_F32;
-    p.Np = (a.N + 7) / 8 * 8;
-    p.drop = drop_key(a.p, a.seed, a.step, a.row_offset, a.state);
-    return p;
-}
-static int norm_rpb(int64_t N) {  // rows a workgroup holds at once
-    int r = 1;
-    (void)by_width((int)std::min<int64_t>(N, LONG_N), [&](auto t, auto, auto b) {
-        r = b.value / t.value;
-        return hipSuccess;
-    });
-    return r;
-}
-// workgroups of the backward = rows of partial weight sums
-static int64_t norm_parts(int64_t M, int64_t N) {
-    if (N > LONG_N) return std::min<int64_t>(M, 32);
-    const int64_t need = (M + norm_rpb(N) - 1) / norm_rpb(N);
-    return std::min<int64_t>(need, N > 8192 ? 256 : 512);
-}
-int64_t norm_bwd_ws(int64_t M, int64_t N) {
-    return norm_parts(std::max<int64_t>(M, 1), N) * 2 * ((N + 7) / 8 * 8) * (int64_t)sizeof(float);
-}
-
 hipError_t norm_fwd(const mmvae_norm_args& a, hipStream_t st) {
     if (a.M == 0) return hipSuccess;
-    NormP p = norm_p(a);
-    p.y = a.y;
-    p.ldy = a.ldy;
-    return by_type(a.dtype, [&](auto ty) -> hipError_t {
-        using T = decltype(ty);
-        if (a.N > LONG_N)
-            return launch(k_ln_fwd_long<T>, dim3((unsigned)std::min<int64_t>(a.M, 512)), dim3(1024), st, p);
-        return by_width(p.N, [&](auto t, auto v, auto b) -> hipError_t {
-            constexpr int RPB = b.value / t.value;
-            const int64_t g = std::min<int64_t>((a.M + RPB - 1) / RPB, 256 * (2048 / b.value));
-            return launch(k_ln_fwd<T, t.value, v.value, b.value>, dim3((unsigned)g), dim3(b.value), st, p);
-        });
-    });
+    return a.dtype == MMVAE_T_F32 ? norm_fwd_f32(a, st) : a.dtype == MMVAE_T_BF16 ? norm_fwd_bf16(a, st) : norm_fwd_f16(a, st);
 }
-
 hipError_t norm_bwd(const mmvae_norm_args& a, hipStream_t st) {
-    NormP p = norm_p(a);
-    p.dy = a.dy;
-    p.lddy = a.lddy;
-    p.y = a.dx;
-    p.ldy = a.lddx;
-    const bool wg = a.dw || a.db;
-    p.part = wg ? (float*)a.ws : nullptr;
-    const int64_t G = norm_parts(a.M, a.N);
-    if (a.M > 0 && (a.dx || wg)) {
-        OPCHK(by_type(a.dtype, [&](auto ty) -> hipError_t {
-            using T = decltype(ty);
-            if (a.N > LONG_N) {
-                if (wg)  // (first: dx may overwrite dy or x)
-                    OPCHK(launch(k_ln_cols<T>, dim3((unsigned)((p.Np / 8 + 255) / 256), (unsigned)G), dim3(256), st, p));
-                return a.dx ? launch(k_ln_bwd_long<T>, dim3((unsigned)std::min<int64_t>(a.M, 512)), dim3(1024), st, p) : hipSuccess;
-            }
-            return by_width(p.N, [&](auto t, auto v, auto b) -> hipError_t {
-                return launch(k_ln_bwd<T, t.value, v.value, b.value>, dim3((unsigned)G), dim3(b.value), st, p);
-            });
-        }));
-    }
-    if (!wg) return hipSuccess;
-    return by_type(a.wtype, [&](auto ty) -> hipError_t {
-        using W = decltype(ty);
-        return launch(k_ln_wred<W>, dim3((unsigned)((2 * p.Np + 63) / 64)), dim3(1024), st, p.N, p.Np, (int)(a.M > 0 ? G : 0),
-                      (const float*)a.ws, (W*)a.dw, (W*)a.db);
-    });
+    return a.dtype == MMVAE_T_F32 ? norm_bwd_f32(a, st) : a.dtype == MMVAE_T_BF16 ? norm_bwd_bf16(a, st) : norm_bwd_f16(a, st);
 }
 
 hipError_t dropout(const mmvae_dropout_args& a, hipStream_t st) {
@@ -1276,7 +653,7 @@ const char* norm_check(const mmvae_norm_args& a, bool bwd) {
     }
     if (a.M > 0 && (!a.dy || !a.mean || !a.rstd)) return "dy, mean or rstd is null";
     if (a.dx && !ld_ok(a.lddx, a.N, a.M)) return "dx's row stride is below N";
-    if ((a.dw || a.db) && (!a.ws || a.ws_bytes < norm_bwd_ws(a.M, a.N))) return "the workspace is below mmvae_layer_norm_bwd_ws(M, N) bytes";
+    if ((a.dw || a.db) && norm_bwd_ws(a.M, a.N) > 0 && (!a.ws || a.ws_bytes < norm_bwd_ws(a.M, a.N))) return "the workspace is below mmvae_layer_norm_bwd_ws(M, N) bytes";
     return nullptr;
 }
 const char* dropout_check(const mmvae_dropout_args& a) {

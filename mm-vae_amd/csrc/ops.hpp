@@ -10,6 +10,13 @@ namespace mmvae {
 hipError_t norm_fwd(const mmvae_norm_args& a, hipStream_t st);
 hipError_t norm_bwd(const mmvae_norm_args& a, hipStream_t st);
 int64_t norm_bwd_ws(int64_t M, int64_t N);
+// one type each (norm_f32 / _bf16 / _f16.hip; M > 0)
+hipError_t norm_fwd_f32(const mmvae_norm_args& a, hipStream_t st);
+hipError_t norm_bwd_f32(const mmvae_norm_args& a, hipStream_t st);
+hipError_t norm_fwd_bf16(const mmvae_norm_args& a, hipStream_t st);
+hipError_t norm_bwd_bf16(const mmvae_norm_args& a, hipStream_t st);
+hipError_t norm_fwd_f16(const mmvae_norm_args& a, hipStream_t st);
+hipError_t norm_bwd_f16(const mmvae_norm_args& a, hipStream_t st);
 hipError_t dropout(const mmvae_dropout_args& a, hipStream_t st);
 hipError_t emb_fwd(const mmvae_embedding_args& a, hipStream_t st);
 hipError_t emb_bwd(const mmvae_embedding_args& a, hipStream_t st);
