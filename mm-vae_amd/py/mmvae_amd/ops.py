@@ -34,84 +34,82 @@ def _wrong(what):
     raise MMVAEError(what)
 
 
-def _rows(t, name, like=None):
-    """t as [rows, N] with unit column stride (a view where it is one); its row stride."""
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
+def _rows(t, name):
+    """t as [rows, N] with unit column stride (a view where it is one)."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         _wrong(f"{name} must be a CUDA tensor")
     if t.dtype not in _TYPE:
         _wrong(f"{name}: float32, bfloat16 or float16, not {t.dtype}")
-    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
-        _wrong(f"{name} must have the shape, type and device of the other tensors")
     if t.dim() == 0 or t.shape[-1] == 0:
         _wrong(f"{name} needs a last dimension of at least 1")
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
     if t.stride(1) != 1 and t.shape[1] > 1:
         t = t.contiguous()
-    return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+    return t
 
 
-def _weight(t, name, x):
-    if t is None:
-        return 0
-    if not isinstance(t, torch.Tensor) or t.device != x.device or t.shape != (x.shape[-1],):
-        _wrong(f"{name} must be a tensor of [{x.shape[-1]}] on x's device")
+def _like(t, name, x):
+    if not isinstance(t, torch.Tensor) or t.shape != x.shape or t.dtype != x.dtype or t.get_device() != x.get_device():
+        _wrong(f"{name} must have the shape, type and device of the other tensors")
+
+
+def _weight(t, name, N, x):
+    """Pointer and type code of a weight or bias."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != x.get_device() or t.dim() != 1 or t.shape[0] != N:
+        _wrong(f"{name} must be a tensor of [{N}] on x's device")
     if t.dtype != x.dtype and t.dtype != torch.float32:
         _wrong(f"{name}: x's type or float32, not {t.dtype}")
-    if t.stride(0) != 1 and t.shape[0] > 1:
+    if not t.is_contiguous():
         _wrong(f"{name} must be contiguous")
-    return t.data_ptr()
+    return t.data_ptr(), _TYPE[t.dtype]
+
+
+def _weights(weight, bias, N, x):
+    """(weight pointer, bias pointer, their type code)"""
+    w = b = 0
+    tw = tb = -1
+    if weight is not None:
+        w, tw = _weight(weight, "weight", N, x)
+    if bias is not None:
+        b, tb = _weight(bias, "bias", N, x)
+        if tw >= 0 and tw != tb:
+            _wrong("weight and bias must have one type")
+    return w, b, max(tw, tb, 0)
 
 
 def _state(state, x):
-    if state is None:
-        return 0
-    if not isinstance(state, torch.Tensor) or state.device != x.device or state.dtype != torch.int64 or state.numel() != 2 or not state.is_contiguous():
+    if (not isinstance(state, torch.Tensor) or state.get_device() != x.get_device() or state.dtype != torch.int64 or state.numel() != 2
+            or not state.is_contiguous()):
         _wrong("state must be a contiguous int64 tensor [step, row_offset] on x's device")
     return state.data_ptr()
 
 
-def _stream(x):
-    return torch.cuda.current_stream(x.device).cuda_stream, x.device.index
-
-
-def _call(name, args):
-    rc = getattr(lib(), name)(args)
-    if rc != 0:
-        _wrong(f"{name} failed ({rc}): {lib().mmvae_last_error(None).decode()}")
-
-
-def _norm_args(x, ldx, w, b, wtype, y=0, ldy=0, mean=0, rstd=0, dy=0, lddy=0, dx=0, lddx=0, dw=0, db=0, ws=0, ws_bytes=0,
-               eps=0.0, relu=False, p=0.0, seed=0, step=0, row_offset=0, state=0):
-    st, dev = _stream(x)
-    return _NORM.pack(x.shape[0], x.shape[1], x.data_ptr(), ldx, w, b, y, ldy, mean, rstd, dy, lddy, dx, lddx, dw, db, ws, ws_bytes,
-                      p, seed & _MASK, step & _MASK, row_offset & _MASK, state, st, dev, _TYPE[x.dtype], wtype, eps, 1 if relu else 0, 0)
-
-
-def _wtype(x, weight, bias):
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        _wrong("weight and bias must have one type")
-    t = weight if weight is not None else bias
-    return _TYPE.get(t.dtype, -1) if t is not None else 0
+def _failed(name, rc):
+    _wrong(f"{name} failed ({rc}): {lib().mmvae_last_error(None).decode()}")
 
 
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, *, relu=False, p=0.0, seed=0, step=0, row_offset=0, state=None, stats=True):
     """y, mean, rstd of drop(relu?(norm(x) * weight + bias)) over x's last dimension; ``stats=False`` (serving)
     stores no statistics and returns None for them."""
-    x2, ldx = _rows(x, "x")
-    w, b = _weight(weight, "weight", x2), _weight(bias, "bias", x2)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    x2 = _rows(x, "x")
     M, N = x2.shape
+    w, b, wtype = _weights(weight, bias, N, x2)
+    y = x.new_empty(x.shape)
     mean = rstd = None
+    pm = pr = 0
     if stats:
-        both = torch.empty((2, M), dtype=torch.float32, device=x.device)
-        mean, rstd = both[0], both[1]
-    _call("mmvae_layer_norm_fwd", _norm_args(
-        x2, ldx, w, b, _wtype(x2, weight, bias), y=y.data_ptr(), ldy=N, mean=mean.data_ptr() if stats else 0,
-        rstd=rstd.data_ptr() if stats else 0, eps=eps, relu=relu, p=p, seed=seed, step=step, row_offset=row_offset,
-        state=_state(state, x2)))
-    if stats and x.dim() != 2:
-        mean, rstd = mean.view(x.shape[:-1]), rstd.view(x.shape[:-1])
+        mean, rstd = x.new_empty(x.shape[:-1], dtype=torch.float32), x.new_empty(x.shape[:-1], dtype=torch.float32)
+        pm, pr = mean.data_ptr(), rstd.data_ptr()
+    dev = x2.get_device()
+    rc = lib().mmvae_layer_norm_fwd(_NORM.pack(
+        M, N, x2.data_ptr(), x2.stride(0), w, b, y.data_ptr(), N, pm, pr, 0, 0, 0, 0, 0, 0, 0, 0, p, seed & _MASK, step & _MASK,
+        row_offset & _MASK, 0 if state is None else _state(state, x2), _raw_stream(dev), dev, _TYPE[x2.dtype], wtype, eps, 1 if relu else 0, 0))
+    if rc:
+        _failed("layer_norm_forward", rc)
     return y, mean, rstd
 
 
@@ -119,78 +117,92 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, bias=None, *, relu=False
                         need=(True, True, True)):
     """dx, dweight, dbias (of weight's type, float32 without one; None where ``need`` says so) from the forward's
     x and statistics; ReLU and dropout as the forward had them (its bias is needed for the ReLU)."""
-    x2, ldx = _rows(x, "x")
-    dy2, lddy = _rows(dy, "dy", x)
-    w, b = _weight(weight, "weight", x2), _weight(bias, "bias", x2)
+    x2 = _rows(x, "x")
+    _like(dy, "dy", x)
+    dy2 = _rows(dy, "dy")
     M, N = x2.shape
-    for t, name in ((mean, "mean"), (rstd, "rstd")):
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != x.device or t.numel() != M or not t.is_contiguous():
-            _wrong(f"{name} must be the forward's float32 statistics")
-    wtype = _wtype(x2, weight, bias)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
-    wt = (weight if weight is not None else bias).dtype if weight is not None or bias is not None else torch.float32
-    dw = torch.empty(N, dtype=wt, device=x.device) if need[1] else None
-    db = torch.empty(N, dtype=wt, device=x.device) if need[2] else None
+    w, b, wtype = _weights(weight, bias, N, x2)
+    dev = x2.get_device()
+    for t in (mean, rstd):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.get_device() != dev or t.numel() != M or not t.is_contiguous():
+            _wrong("mean and rstd must be the forward's float32 statistics")
+    wt = weight if weight is not None else bias
+    wt = torch.float32 if wt is None else wt.dtype
+    dx = x.new_empty(x.shape) if need[0] else None
+    dw = x.new_empty((N,), dtype=wt) if need[1] else None
+    db = x.new_empty((N,), dtype=wt) if need[2] else None
     ws, n = None, 0
     if need[1] or need[2]:
         n = lib().mmvae_layer_norm_bwd_ws(M, N)
-        ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-    _call("mmvae_layer_norm_bwd", _norm_args(
-        x2, ldx, w, b, wtype, mean=mean.data_ptr(), rstd=rstd.data_ptr(), dy=dy2.data_ptr(), lddy=lddy,
-        dx=dx.data_ptr() if need[0] else 0, lddx=N, dw=dw.data_ptr() if need[1] else 0, db=db.data_ptr() if need[2] else 0,
-        ws=ws.data_ptr() if n else 0, ws_bytes=n, relu=relu, p=p, seed=seed, step=step, row_offset=row_offset, state=_state(state, x2)))
+        if n:
+            ws = x.new_empty((n,), dtype=torch.uint8)
+    rc = lib().mmvae_layer_norm_bwd(_NORM.pack(
+        M, N, x2.data_ptr(), x2.stride(0), w, b, 0, 0, mean.data_ptr(), rstd.data_ptr(), dy2.data_ptr(), dy2.stride(0),
+        dx.data_ptr() if need[0] else 0, N, dw.data_ptr() if need[1] else 0, db.data_ptr() if need[2] else 0, ws.data_ptr() if n else 0, n,
+        p, seed & _MASK, step & _MASK, row_offset & _MASK, 0 if state is None else _state(state, x2), _raw_stream(dev), dev, _TYPE[x2.dtype],
+        wtype, 0.0, 1 if relu else 0, 0))
+    if rc:
+        _failed("layer_norm_backward", rc)
     return dx, dw, db
 
 
 def dropout_apply(x, p, seed, *, step=0, row_offset=0, state=None):
     """x with each element dropped with probability p, or scaled by 1 / P(kept); on dy: the gradient."""
-    x2, ldx = _rows(x, "x")
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    st, dev = _stream(x2)
-    _call("mmvae_dropout", _DROP.pack(x2.shape[0], x2.shape[1], x2.data_ptr(), ldx, y.data_ptr(), x2.shape[1], p, seed & _MASK,
-                                      step & _MASK, row_offset & _MASK, _state(state, x2), st, dev, _TYPE[x.dtype]))
+    x2 = _rows(x, "x")
+    y = x.new_empty(x.shape)
+    M, N = x2.shape
+    dev = x2.get_device()
+    rc = lib().mmvae_dropout(_DROP.pack(M, N, x2.data_ptr(), x2.stride(0), y.data_ptr(), N, p, seed & _MASK, step & _MASK, row_offset & _MASK,
+                                        0 if state is None else _state(state, x2), _raw_stream(dev), dev, _TYPE[x2.dtype]))
+    if rc:
+        _failed("dropout_apply", rc)
     return y
 
 
-def _ids(ids, device):
-    if not isinstance(ids, torch.Tensor) or ids.dtype not in (torch.int64, torch.int32) or ids.device != device:
+def _ids(ids, t):
+    if not isinstance(ids, torch.Tensor) or ids.dtype not in (torch.int64, torch.int32) or ids.get_device() != t.get_device():
         _wrong("ids must be an int64 or int32 tensor on the table's device")
-    return ids.contiguous()
+    return ids if ids.is_contiguous() else ids.contiguous()
 
 
 def embedding_forward(ids, table, scale=1.0, add=None):
     """scale * table[ids] (+ add), ids of any shape; an id outside [0, rows) looks up zeros."""
-    t2, ldt = _rows(table, "table")
+    t2 = _rows(table, "table")
     if table.dim() != 2:
         _wrong("table must be [rows, N]")
-    i = _ids(ids, table.device)
-    N = t2.shape[1]
-    y = torch.empty((*ids.shape, N), dtype=table.dtype, device=table.device)
-    a, lda = 0, 0
+    i = _ids(ids, t2)
+    V, N = t2.shape
+    y = t2.new_empty((*ids.shape, N))
+    a = lda = 0
     if add is not None:
-        a2, lda = _rows(add, "add", y)
-        a = a2.data_ptr()
-    st, dev = _stream(t2)
-    _call("mmvae_embedding_fwd", _EMB.pack(i.numel(), N, t2.shape[0], i.data_ptr(), t2.data_ptr(), ldt, a, lda, y.data_ptr(), N, 0, 0, 0, 0,
-                                           0, st, dev, _TYPE[table.dtype], 1 if i.dtype == torch.int64 else 0, scale))
+        _like(add, "add", y)
+        add = _rows(add, "add")
+        a, lda = add.data_ptr(), add.stride(0)
+    dev = t2.get_device()
+    rc = lib().mmvae_embedding_fwd(_EMB.pack(i.numel(), N, V, i.data_ptr(), t2.data_ptr(), t2.stride(0), a, lda, y.data_ptr(), N, 0, 0, 0, 0, 0,
+                                             _raw_stream(dev), dev, _TYPE[t2.dtype], 1 if i.dtype == torch.int64 else 0, scale))
+    if rc:
+        _failed("embedding_forward", rc)
     return y
 
 
 def embedding_backward(dy, ids, rows, scale=1.0):
     """The table's gradient [rows, N] in dy's type: scale times the sum of dy over each row's tokens."""
-    d2, lddy = _rows(dy, "dy")
-    i = _ids(ids, dy.device)
+    d2 = _rows(dy, "dy")
+    i = _ids(ids, d2)
     T, N = i.numel(), dy.shape[-1]
     if dy.shape[:-1] != ids.shape:
         _wrong("dy must be ids' shape and the width")
     if not isinstance(rows, int) or rows < 0:
         _wrong("rows must be the table's row count")
-    out = torch.empty((rows, N), dtype=dy.dtype, device=dy.device)
+    out = d2.new_empty((rows, N))
     n = lib().mmvae_embedding_bwd_ws(T, N)
-    ws = torch.empty(n, dtype=torch.uint8, device=dy.device)
-    st, dev = _stream(d2)
-    _call("mmvae_embedding_bwd", _EMB.pack(T, N, rows, i.data_ptr(), 0, 0, 0, 0, 0, 0, d2.data_ptr(), lddy, out.data_ptr(), ws.data_ptr(), n,
-                                           st, dev, _TYPE[dy.dtype], 1 if i.dtype == torch.int64 else 0, scale))
+    ws = d2.new_empty((n,), dtype=torch.uint8)
+    dev = d2.get_device()
+    rc = lib().mmvae_embedding_bwd(_EMB.pack(T, N, rows, i.data_ptr(), 0, 0, 0, 0, 0, 0, d2.data_ptr(), d2.stride(0), out.data_ptr(), ws.data_ptr(), n,
+                                             _raw_stream(dev), dev, _TYPE[d2.dtype], 1 if i.dtype == torch.int64 else 0, scale))
+    if rc:
+        _failed("embedding_backward", rc)
     return out
 
 

@@ -76,7 +76,8 @@ def test_norm_forward_refuses(kw):
     assert L.mmvae_last_error(None).startswith(b"layer_norm_fwd: ")
 
 
-@pytest.mark.parametrize("kw", NORM_BAD + [dict(dy=0), dict(mean=0), dict(rstd=0), dict(lddx=7), dict(ws=0), dict(ws_bytes=8), dict(lddy=-8)])
+@pytest.mark.parametrize("kw", NORM_BAD + [dict(dy=0), dict(mean=0), dict(rstd=0), dict(lddx=7), dict(M=5000, ws=0),
+                                            dict(M=5000, ws_bytes=8), dict(lddy=-8)])
 def test_norm_backward_refuses(kw):
     assert mmvae_amd.lib().mmvae_layer_norm_bwd(pack_norm(**kw)) == -1
 
@@ -110,8 +111,10 @@ def test_workspace_sizes_grow_with_the_call():
     assert L.mmvae_layer_norm_bwd_ws(-1, 8) == 0 and L.mmvae_layer_norm_bwd_ws(4, 0) == 0
     assert L.mmvae_embedding_bwd_ws(-1, 8) == 0 and L.mmvae_embedding_bwd_ws(4, 0) == 0
     for N in (1, 7, 64, 100, 1000, 20000, 32768, 32769, 100000):
-        for M in (0, 1, 2, 100, 4096):
-            assert L.mmvae_layer_norm_bwd_ws(M, N) >= 2 * 4 * N
+        for M in (0, 1, 2, 100, 4096):  # few rows: one workgroup, no partial sums
+            n = L.mmvae_layer_norm_bwd_ws(M, N)
+            assert n >= 2 * 2 * 4 * N or (n == 0 and M <= (256 if N <= 1024 else 1)) or (N > 32768 and n >= 2 * 4 * N)
+        assert L.mmvae_layer_norm_bwd_ws(4096, N) > 0
     # two sorted copies of the tokens (id, position), and a partial head and tail of a piece at least
     for T in (1, 4096, 4097, 600000):
         assert L.mmvae_embedding_bwd_ws(T, 33) >= 16 * T + 2 * 4 * 40
