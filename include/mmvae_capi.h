@@ -354,7 +354,7 @@ typedef struct mmvae_embedding_args {
     const void *dy;            /* backward */
     int64_t lddy;
     void *dtable;
-    void *ws;                  /* backward: mmvae_embedding_bwd_ws(T, N) bytes */
+    void *ws;                  /* backward: mmvae_embedding_bwd_ws(T, N, V) bytes, 16-byte aligned */
     int64_t ws_bytes;
     void *stream;
     int32_t device;
@@ -364,7 +364,7 @@ typedef struct mmvae_embedding_args {
 } mmvae_embedding_args;
 int mmvae_embedding_fwd(const mmvae_embedding_args* args);
 int mmvae_embedding_bwd(const mmvae_embedding_args* args);
-int64_t mmvae_embedding_bwd_ws(int64_t T, int64_t N);
+int64_t mmvae_embedding_bwd_ws(int64_t T, int64_t N, int64_t V);
 
 /* ---- operators.hh (vMF observation model scalars) ----------------------------------
  * lbessel(kappa, nu): piecewise log I_nu(kappa) approximation (operators.hh:49-101) with

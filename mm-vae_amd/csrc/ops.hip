@@ -12,25 +12,52 @@
 namespace mmvae {
 
 // =======================================================================================
-// Dropout alone: tpr = 2^s threads walk a row's chunks, 256 / tpr rows per workgroup
+// Chunks of many rows, dealt out evenly whatever the width: chunk i of all is chunk i % nc of row
+// i / nc.  A workgroup takes 1024 in a row, four a thread (their loads in flight together); the
+// division is once per workgroup, and within it by a float product (li + 1/2) / nc, whose distance
+// from a whole number, >= 1 / (2 nc), is above its error for li < 2^22 (N < 2^24, or one row's part).
+// =======================================================================================
+static constexpr int WALK = 4;
+struct Walk {
+    int64_t row0;  // the workgroup's first chunk: its row and place there
+    int c0;
+    float inv;
+    int nc;
+};
+MMVAE_DEV Walk walk_from(int64_t nc) {
+    const int64_t i = (int64_t)blockIdx.x * (256 * WALK), r = i / nc;
+    return Walk{r, (int)(i - r * nc), 1.f / (float)nc, (int)nc};
+}
+MMVAE_DEV int64_t walk_row(const Walk& w, int u, int* chunk) {
+    const int li = w.c0 + u * 256 + (int)threadIdx.x, q = (int)(((float)li + 0.5f) * w.inv);
+    *chunk = li - q * w.nc;
+    return w.row0 + q;
+}
+static int64_t walk_blocks(int64_t rows, int64_t N) { return (rows * ((N + 7) / 8) + 256 * WALK - 1) / (256 * WALK); }
+
+// =======================================================================================
+// Dropout alone
 // =======================================================================================
 template <class T>
-__global__ __launch_bounds__(256) void k_dropout(int64_t M, int64_t N, const T* x, int64_t ldx, T* y, int64_t ldy, int ltpr, DropKey k) {
-    const int tpr = 1 << ltpr, rpb = 256 >> ltpr;
-    const int lane = threadIdx.x & (tpr - 1), grp = threadIdx.x >> ltpr;
+__global__ __launch_bounds__(256) void k_dropout(int64_t M, int N, const T* x, int64_t ldx, T* y, int64_t ldy, DropKey k) {
     drop_state(k);
-    for (int64_t row = (int64_t)blockIdx.x * rpb + grp; row < M; row += (int64_t)gridDim.x * rpb) {
-        const T* xr = x + row * ldx;
-        T* yr = y + row * ldy;
-        for (int64_t col = lane * 8; col < N; col += tpr * 8) {
-            const int n = (int)(N - col < 8 ? N - col : 8);
-            Chunk<T> c = ld8(xr + col, n);
-            bool kept[8];
-            keep8(k, row, (int)(col >> 3), kept);
+    const Walk w = walk_from((N + 7) / 8);
+    int c[WALK];
+    int64_t row[WALK];
+    Chunk<T> v[WALK];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) c.set(i, kept[i] ? c.get(i) * k.s : 0.f);
-            st8(yr + col, n, c);
-        }
+    for (int u = 0; u < WALK; ++u) {
+        row[u] = walk_row(w, u, &c[u]);
+        v[u] = ld8(x + (row[u] < M ? row[u] : 0) * ldx + c[u] * 8, N - c[u] * 8);
+    }
+#pragma unroll
+    for (int u = 0; u < WALK; ++u) {
+        if (row[u] >= M) break;
+        bool kept[8];
+        keep8(k, row[u], c[u], kept);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[u].set(i, kept[i] ? v[u].get(i) * k.s : 0.f);
+        st8(y + row[u] * ldy + c[u] * 8, N - c[u] * 8, v[u]);
     }
 }
 
@@ -50,51 +77,66 @@ struct EmbF {
 MMVAE_DEV int64_t emb_id(const void* ids, int i64, int64_t t) {
     return i64 ? ((const int64_t*)ids)[t] : (int64_t)((const int32_t*)ids)[t];
 }
-template <class T> __global__ __launch_bounds__(256) void k_emb_fwd(EmbF a, int ltpr) {
-    const int tpr = 1 << ltpr, rpb = 256 >> ltpr;
-    const int lane = threadIdx.x & (tpr - 1), grp = threadIdx.x >> ltpr;
-    for (int64_t t = (int64_t)blockIdx.x * rpb + grp; t < a.T; t += (int64_t)gridDim.x * rpb) {
-        const int64_t id = emb_id(a.ids, a.i64, t);
-        const bool ok = id >= 0 && id < a.V;
-        const T* tr = (const T*)a.table + (ok ? id : 0) * a.ldt;
-        T* yr = (T*)a.y + t * a.ldy;
-        for (int col = lane * 8; col < a.N; col += tpr * 8) {
-            const int n = a.N - col;
-            Chunk<T> c = ld8(tr + col, ok ? n : 0);
-            if (a.add) {
-                const Chunk<T> d = ld8((const T*)a.add + t * a.ldadd + col, n);
+template <class T> __global__ __launch_bounds__(256) void k_emb_fwd(EmbF a) {
+    const Walk w = walk_from((a.N + 7) / 8);
+    int c[WALK];
+    int64_t t[WALK], id[WALK];
+    Chunk<T> v[WALK];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) c.set(i, ok ? __builtin_fmaf(c.get(i), a.scale, d.get(i)) : d.get(i));
-            } else {
+    for (int u = 0; u < WALK; ++u) {
+        t[u] = walk_row(w, u, &c[u]);
+        id[u] = emb_id(a.ids, a.i64, t[u] < a.T ? t[u] : 0);
+    }
 #pragma unroll
-                for (int i = 0; i < 8; ++i) c.set(i, ok ? c.get(i) * a.scale : 0.f);
-            }
-            st8(yr + col, n, c);
+    for (int u = 0; u < WALK; ++u) {
+        const bool ok = id[u] >= 0 && id[u] < a.V;
+        v[u] = ld8((const T*)a.table + (ok ? id[u] : 0) * a.ldt + c[u] * 8, ok ? a.N - c[u] * 8 : 0);
+    }
+#pragma unroll
+    for (int u = 0; u < WALK; ++u) {
+        if (t[u] >= a.T) break;
+        const bool ok = id[u] >= 0 && id[u] < a.V;
+        const int col = c[u] * 8, n = a.N - col;
+        if (a.add) {
+            const Chunk<T> d = ld8((const T*)a.add + t[u] * a.ldadd + col, n);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[u].set(i, ok ? __builtin_fmaf(v[u].get(i), a.scale, d.get(i)) : d.get(i));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[u].set(i, ok ? v[u].get(i) * a.scale : 0.f);
         }
+        st8((T*)a.y + t[u] * a.ldy + col, n, v[u]);
     }
 }
 
 // =======================================================================================
 // Embedding gradient: dE[v] = scale sum over the tokens of v of dy.
+// Many table rows (V > FEW):
 //   1. the tokens sorted by id, stable (LSD radix sort, 8-bit digits; ids outside [0, V) as V,
 //      behind all others): in one workgroup up to 4096 tokens, else histogram + scatter per digit;
 //   2. k_emb_seg: fixed pieces of the sorted tokens, whatever their ids: a hot id is spread over
 //      many workgroups, the sums of runs inside a piece are final, the first and last run of a
 //      piece leave a partial where they go on in the next one;
 //   3. k_emb_join: the partials of a run that crosses pieces, summed in order.
+// Few rows (labels: V <= FEW), where a sort of all tokens would cost more than their sums: each
+// piece sorts its own tokens and leaves one partial per row it has (k_emb_seg<FEW>), and
+// k_emb_few_join adds them up in order.
 // =======================================================================================
-static constexpr int RTILE = 4096, RTHR = 1024, RKPT = RTILE / RTHR;  // a sort tile: 16 waves x 4 x 64 tokens
-static constexpr int RFUSE = 128;  // up to so many tiles a scatter workgroup sums the histograms itself
+static constexpr int FEW = 64;
+static constexpr int RTHR = 1024;   // a sort tile: 16 waves x KPT x 64 tokens
+static constexpr int RONE = 4096;   // tokens that one workgroup sorts (KPT = 4)
+static constexpr int RTILE = 2048;  // a tile of a longer sort (KPT = 2)
+static constexpr int RFUSE = 256;   // up to so many tiles a scatter workgroup sums the histograms itself
 
-// stable ranks of the workgroup's keys by an 8-bit digit (16 waves, RKPT keys a lane; wave w holds the
-// tokens w 256 + k 64 + lane).  wh[w][d]: first the wave's counts, then the count of d in earlier waves.
+// stable ranks of the workgroup's keys by an 8-bit digit (16 waves, KPT keys a lane; wave w holds the
+// tokens w 64 KPT + k 64 + lane).  wh[w][d]: first the wave's counts, then the count of d in earlier waves.
 struct RadixLds {
     uint32_t wh[RTHR / 64][256];
     uint32_t tot[256];   // the tile's count of each digit
     uint32_t base[256];  // exclusive sums of tot
     uint32_t ws[4];
 };
-MMVAE_DEV void radix_rank(const uint32_t dig[RKPT], const bool val[RKPT], uint32_t rank[RKPT], RadixLds& L) {
+template <int RKPT> MMVAE_DEV void radix_rank(const uint32_t dig[RKPT], const bool val[RKPT], uint32_t rank[RKPT], RadixLds& L) {
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
     for (int i = threadIdx.x; i < (RTHR / 64) * 256; i += RTHR) L.wh[i >> 8][i & 255] = 0;
     __syncthreads();
@@ -119,11 +161,13 @@ MMVAE_DEV void radix_rank(const uint32_t dig[RKPT], const bool val[RKPT], uint32
     __syncthreads();
     uint32_t t = 0;
     if (threadIdx.x < 256) {
+        uint32_t c[RTHR / 64];
+#pragma unroll
+        for (int q = 0; q < RTHR / 64; ++q) c[q] = L.wh[q][threadIdx.x];
 #pragma unroll
         for (int q = 0; q < RTHR / 64; ++q) {
-            const uint32_t c = L.wh[q][threadIdx.x];
             L.wh[q][threadIdx.x] = t;
-            t += c;
+            t += c[q];
         }
         L.tot[threadIdx.x] = t;
     }
@@ -153,79 +197,78 @@ MMVAE_DEV uint32_t emb_key(const void* ids, int i64, int64_t t, uint32_t V) {
     const int64_t id = emb_id(ids, i64, t);
     return id >= 0 && id < (int64_t)V ? (uint32_t)id : V;
 }
-MMVAE_DEV void fill_zero(uint32_t* out, int64_t words, int64_t i, int64_t step) {  // out 4-byte aligned
-    for (; i < words; i += step) out[i] = 0;
+// bytes of zeros (out 4-byte aligned), by thread i of `step`
+MMVAE_DEV void fill_zero(void* out, int64_t bytes, int64_t i, int64_t step) {
+    const int64_t head = ((16 - ((uintptr_t)out & 15)) & 15) < bytes ? (16 - ((uintptr_t)out & 15)) & 15 : bytes;
+    uint4* q = reinterpret_cast<uint4*>((char*)out + head);
+    const int64_t n = (bytes - head) / 16, rest = bytes - head - n * 16;
+    if (i < head / 4) ((uint32_t*)out)[i] = 0;
+    if (i < rest / 2) ((uint16_t*)(q + n))[i] = 0;
+    if (i == 0 && (head & 2)) ((uint16_t*)out)[head / 2 - 1] = 0;  // (a buffer that ends before its first 16 bytes)
+    for (; i < n; i += step) q[i] = make_uint4(0, 0, 0, 0);
 }
 
-// the whole sort of T <= RTILE tokens in workgroup 0; the others clear the gradient
-__global__ __launch_bounds__(RTHR) void k_emb_sort1(const void* ids, int i64, int T, uint32_t V, int passes, uint32_t* key,
-                                                    uint32_t* idx, void* out, int64_t out_bytes) {
+// the whole sort of T <= RONE tokens in workgroup 0; the others clear the gradient
+__global__ __launch_bounds__(RTHR) void k_emb_sort1(const void* ids, int i64, int T, uint32_t V, int passes, uint2* kv, void* out,
+                                                    int64_t out_bytes) {
     if (blockIdx.x > 0) {
-        fill_zero((uint32_t*)out, out_bytes / 4, (int64_t)(blockIdx.x - 1) * RTHR + threadIdx.x, (int64_t)(gridDim.x - 1) * RTHR);
-        if (blockIdx.x == 1 && threadIdx.x == 0 && (out_bytes & 2)) ((uint16_t*)out)[out_bytes / 2 - 1] = 0;
+        fill_zero(out, out_bytes, (int64_t)(blockIdx.x - 1) * RTHR + threadIdx.x, (int64_t)(gridDim.x - 1) * RTHR);
         return;
     }
+    constexpr int KPT = RONE / RTHR;
     __shared__ RadixLds L;
-    __shared__ uint32_t sk[RTILE], si[RTILE];
+    __shared__ uint2 sh[RONE];
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    uint32_t kk[RKPT], ii[RKPT], dig[RKPT], rank[RKPT];
-    bool val[RKPT];
+    uint32_t kk[KPT], ii[KPT], dig[KPT], rank[KPT];
+    bool val[KPT];
 #pragma unroll
-    for (int k = 0; k < RKPT; ++k) {
-        const int t = w * 256 + k * 64 + lane;
+    for (int k = 0; k < KPT; ++k) {
+        const int t = (w * KPT + k) * 64 + lane;
         val[k] = t < T;
         kk[k] = val[k] ? emb_key(ids, i64, t, V) : 0;
         ii[k] = t;
     }
     for (int p = 0; p < passes; ++p) {
 #pragma unroll
-        for (int k = 0; k < RKPT; ++k) dig[k] = (kk[k] >> (8 * p)) & 255;
-        radix_rank(dig, val, rank, L);
+        for (int k = 0; k < KPT; ++k) dig[k] = (kk[k] >> (8 * p)) & 255;
+        radix_rank<KPT>(dig, val, rank, L);
         digit_scan(L.tot, L);
 #pragma unroll
-        for (int k = 0; k < RKPT; ++k)
-            if (val[k]) {
-                const uint32_t pos = L.base[dig[k]] + L.wh[w][dig[k]] + rank[k];
-                sk[pos] = kk[k];
-                si[pos] = ii[k];
-            }
+        for (int k = 0; k < KPT; ++k)
+            if (val[k]) sh[L.base[dig[k]] + L.wh[w][dig[k]] + rank[k]] = make_uint2(kk[k], ii[k]);
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < RKPT; ++k) {
-            const int t = w * 256 + k * 64 + lane;
+        for (int k = 0; k < KPT; ++k) {
+            const int t = (w * KPT + k) * 64 + lane;
             if (t < T) {
-                kk[k] = sk[t];
-                ii[k] = si[t];
+                kk[k] = sh[t].x;
+                ii[k] = sh[t].y;
             }
         }
     }
 #pragma unroll
-    for (int k = 0; k < RKPT; ++k) {
-        const int t = w * 256 + k * 64 + lane;
-        if (t < T) {
-            key[t] = kk[k];
-            idx[t] = ii[k];
-        }
+    for (int k = 0; k < KPT; ++k) {
+        const int t = (w * KPT + k) * 64 + lane;
+        if (t < T) kv[t] = make_uint2(kk[k], ii[k]);
     }
 }
 
-// digit counts of each tile: hist[tile][256]; key null: the first pass, from the ids.  Workgroups past
+// digit counts of each tile: hist[tile][256]; kv null: the first pass, from the ids.  Workgroups past
 // the tiles (first pass) clear the gradient.
-__global__ __launch_bounds__(RTHR) void k_emb_hist(const void* ids, int i64, const uint32_t* key, int64_t T, uint32_t V, int shift,
-                                                   int tiles, uint32_t* hist, void* out, int64_t out_bytes) {
+__global__ __launch_bounds__(RTHR) void k_emb_hist(const void* ids, int i64, const uint2* kv, int64_t T, uint32_t V, int shift, int tiles,
+                                                   uint32_t* hist, void* out, int64_t out_bytes) {
     if ((int)blockIdx.x >= tiles) {
         const int b = blockIdx.x - tiles, nb = gridDim.x - tiles;
-        fill_zero((uint32_t*)out, out_bytes / 4, (int64_t)b * RTHR + threadIdx.x, (int64_t)nb * RTHR);
-        if (b == 0 && threadIdx.x == 0 && (out_bytes & 2)) ((uint16_t*)out)[out_bytes / 2 - 1] = 0;
+        fill_zero(out, out_bytes, (int64_t)b * RTHR + threadIdx.x, (int64_t)nb * RTHR);
         return;
     }
     __shared__ uint32_t h[256];
     if (threadIdx.x < 256) h[threadIdx.x] = 0;
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < RKPT; ++k) {
+    for (int k = 0; k < RTILE / RTHR; ++k) {
         const int64_t t = (int64_t)blockIdx.x * RTILE + k * RTHR + threadIdx.x;
-        if (t < T) atomicAdd(&h[((key ? key[t] : emb_key(ids, i64, t, V)) >> shift) & 255], 1u);
+        if (t < T) atomicAdd(&h[((kv ? kv[t].x : emb_key(ids, i64, t, V)) >> shift) & 255], 1u);
     }
     __syncthreads();
     if (threadIdx.x < 256) hist[(int64_t)blockIdx.x * 256 + threadIdx.x] = h[threadIdx.x];
@@ -258,12 +301,27 @@ __global__ __launch_bounds__(256) void k_emb_scan(int tiles, uint32_t* hist) {
     }
     if (threadIdx.x == 0) hist[(int64_t)tiles * 256 + d] = carry;
 }
-__global__ __launch_bounds__(RTHR) void k_emb_scatter(const void* ids, int i64, const uint32_t* key, const uint32_t* idx, int64_t T,
-                                                      uint32_t V, int shift, int tiles, int scanned, const uint32_t* hist,
-                                                      uint32_t* key2, uint32_t* idx2) {
+// one pass: a tile's tokens, sorted by the digit in LDS first (so that a digit's tokens leave together),
+// to their places
+__global__ __launch_bounds__(RTHR) void k_emb_scatter(const void* ids, int i64, const uint2* kv, int64_t T, uint32_t V, int shift, int tiles,
+                                                      int scanned, const uint32_t* hist, uint2* kv2) {
+    constexpr int KPT = RTILE / RTHR;
     __shared__ RadixLds L;
     __shared__ uint32_t pre[4][256], all[4][256];
+    __shared__ uint2 sh[RTILE];
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t t0 = (int64_t)blockIdx.x * RTILE;
+    uint32_t kk[KPT], ii[KPT], dig[KPT], rank[KPT];
+    bool val[KPT];
+#pragma unroll
+    for (int k = 0; k < KPT; ++k) {
+        const int64_t t = t0 + (w * KPT + k) * 64 + lane;
+        val[k] = t < T;
+        uint2 v = make_uint2(0, 0);
+        if (val[k]) v = kv ? kv[t] : make_uint2(emb_key(ids, i64, t, V), (uint32_t)t);
+        kk[k] = v.x;
+        ii[k] = v.y;
+    }
     {  // the digits' totals and their counts in earlier tiles
         const int d = threadIdx.x & 255, q = threadIdx.x >> 8;
         uint32_t p = 0, t = 0;
@@ -273,41 +331,41 @@ __global__ __launch_bounds__(RTHR) void k_emb_scatter(const void* ids, int i64, 
                 t = hist[(int64_t)tiles * 256 + d];
             }
         } else {
-            for (int b = q; b < tiles; b += 4) {
-                const uint32_t v = hist[(int64_t)b * 256 + d];
-                t += v;
-                if (b < (int)blockIdx.x) p += v;
+            for (int b0 = q; b0 < tiles; b0 += 64) {  // 16 loads in flight
+                uint32_t v[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) v[k] = hist[(int64_t)min(b0 + 4 * k, tiles - 1) * 256 + d];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const int b = b0 + 4 * k;
+                    t += b < tiles ? v[k] : 0;
+                    p += b < (int)blockIdx.x ? v[k] : 0;
+                }
             }
         }
         pre[q][d] = p;
         all[q][d] = t;
     }
-    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < KPT; ++k) dig[k] = (kk[k] >> shift) & 255;
+    radix_rank<KPT>(dig, val, rank, L);  // (its barriers cover pre and all)
+    digit_scan(L.tot, L);                // base: the digit's first place in the tile
+#pragma unroll
+    for (int k = 0; k < KPT; ++k)
+        if (val[k]) sh[L.base[dig[k]] + L.wh[w][dig[k]] + rank[k]] = make_uint2(kk[k], ii[k]);
     if (threadIdx.x < 256) {
         const int d = threadIdx.x;
-        pre[0][d] = pre[0][d] + pre[1][d] + pre[2][d] + pre[3][d];
+        pre[0][d] = pre[0][d] + pre[1][d] + pre[2][d] + pre[3][d] - L.base[d];
         all[0][d] = all[0][d] + all[1][d] + all[2][d] + all[3][d];
     }
     __syncthreads();
-    digit_scan(all[0], L);
-    uint32_t kk[RKPT], ii[RKPT], dig[RKPT], rank[RKPT];
-    bool val[RKPT];
-#pragma unroll
-    for (int k = 0; k < RKPT; ++k) {
-        const int64_t t = (int64_t)blockIdx.x * RTILE + w * 256 + k * 64 + lane;
-        val[k] = t < T;
-        kk[k] = val[k] ? (key ? key[t] : emb_key(ids, i64, t, V)) : 0;
-        ii[k] = val[k] && idx ? idx[t] : (uint32_t)t;
-        dig[k] = (kk[k] >> shift) & 255;
+    digit_scan(all[0], L);  // base: the digit's first place of all
+    const int n = T - t0 < RTILE ? (int)(T - t0) : RTILE;
+    for (int j = threadIdx.x; j < n; j += RTHR) {
+        const uint2 v = sh[j];
+        const uint32_t d = (v.x >> shift) & 255;
+        kv2[L.base[d] + pre[0][d] + (uint32_t)j] = v;  // (modulo 2^32: pre may be "negative")
     }
-    radix_rank(dig, val, rank, L);
-#pragma unroll
-    for (int k = 0; k < RKPT; ++k)
-        if (val[k]) {
-            const uint32_t pos = L.base[dig[k]] + pre[0][dig[k]] + L.wh[w][dig[k]] + rank[k];
-            key2[pos] = kk[k];
-            idx2[pos] = ii[k];
-        }
 }
 
 struct EmbB {
@@ -315,13 +373,17 @@ struct EmbB {
     int N;
     int64_t Np;
     uint32_t V;
-    const uint32_t *key, *idx;
+    const uint2* kv;  // the sorted tokens: id, place
+    const void* ids;  // FEW: the tokens as they come
+    int i64;
     const void* dy;
     int64_t lddy;
     void* out;
-    float* part;  // [pieces][2][Np]: a piece's head (run from earlier pieces) and tail (run going on)
+    float* part;      // [pieces][2][Np]: a piece's head (run from earlier pieces) and tail (run going on);
+                      // FEW: [pieces][V][Np], the rows that the piece has
+    uint32_t* cnt;    // FEW: [pieces][V] how many tokens
     float scale;
-    int tg;       // tokens per group
+    int tg;           // tokens per group
 };
 template <class T> MMVAE_DEV void emb_out(const EmbB& a, uint32_t key, int col, const float s[8]) {
     if (key >= a.V) return;
@@ -330,46 +392,139 @@ template <class T> MMVAE_DEV void emb_out(const EmbB& a, uint32_t key, int col, 
     for (int i = 0; i < 8; ++i) c.set(i, s[i] * a.scale);
     st8((T*)a.out + (int64_t)key * a.N + col, a.N - col, c);
 }
+static constexpr int PIECE = 1024;  // tokens of a piece at most (FEW: 512)
+static constexpr uint32_t NO_KEY = 0xFFFFFFFFu;
+// the piece's tokens sorted by id (V <= FEW; 256 threads, two tokens each); returns how many have a row
+struct FewLds {
+    uint32_t wh[4][FEW + 1], base[FEW + 1];
+};
+MMVAE_DEV int few_sort(const EmbB& a, int64_t p0, int P, uint32_t* sk, uint32_t* si, FewLds& L) {
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    for (int i = threadIdx.x; i < 4 * (FEW + 1); i += 256) L.wh[i / (FEW + 1)][i % (FEW + 1)] = 0;
+    __syncthreads();
+    uint32_t kk[2], rank[2];
+    bool val[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int j = w * 128 + k * 64 + lane;
+        val[k] = j < P && p0 + j < a.T;
+        kk[k] = val[k] ? emb_key(a.ids, a.i64, p0 + j, a.V) : 0;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        uint64_t m = __ballot(val[k]);
+#pragma unroll
+        for (int b = 0; b < 7; ++b) {
+            const bool bit = (kk[k] >> b) & 1;
+            const uint64_t bal = __ballot(bit);
+            m &= bit ? bal : ~bal;
+        }
+        const uint32_t lt = __popcll(m & ((uint64_t(1) << lane) - 1));
+        const uint32_t old = val[k] ? L.wh[w][kk[k]] : 0;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (val[k] && lt == 0) L.wh[w][kk[k]] = old + __popcll(m);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        rank[k] = old + lt;
+    }
+    __syncthreads();
+    if (threadIdx.x < 64) {  // ids 0 .. 63: the waves' counts to offsets, then the ids'
+        uint32_t t = 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const uint32_t c = L.wh[q][threadIdx.x];
+            L.wh[q][threadIdx.x] = t;
+            t += c;
+        }
+        const uint32_t own = t;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t u = __shfl_up(t, o, 64);
+            if (lane >= o) t += u;
+        }
+        L.base[threadIdx.x] = t - own;
+        if (threadIdx.x == 63) L.base[FEW] = t;
+        if (blockIdx.y == 0 && threadIdx.x < a.V) a.cnt[(int64_t)blockIdx.x * a.V + threadIdx.x] = threadIdx.x < (uint32_t)a.V ? own : 0;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        if (val[k] && kk[k] < a.V) {
+            const uint32_t pos = L.base[kk[k]] + L.wh[w][kk[k]] + rank[k];
+            sk[1 + pos] = kk[k];
+            si[pos] = (uint32_t)(p0 + w * 128 + k * 64 + lane);
+        }
+    // (with V = FEW the ids outside count as FEW, with V < FEW as V: behind the rows either way)
+    return (int)(a.V < FEW ? L.base[a.V] : L.base[FEW]);
+}
 // TPR lanes x 8 columns; the 256 / TPR groups of a workgroup take a.tg consecutive sorted tokens each
-template <class T, int TPR> __global__ __launch_bounds__(256) void k_emb_seg(EmbB a) {
+template <class T, int TPR, bool ISFEW> __global__ __launch_bounds__(256) void k_emb_seg(EmbB a) {
     constexpr int GB = 256 / TPR, U = 8;
     __shared__ float head[GB][TPR * 8], tail[GB][TPR * 8];
-    __shared__ uint32_t first[GB], last[GB];  // a group's first and last key
+    __shared__ uint32_t last[GB];             // a group's last key
     __shared__ int hflag[GB], tflag[GB];      // first run goes on from before; last run goes on behind (2: one run, from before)
+    __shared__ uint32_t sk[(ISFEW ? 512 : PIECE) + 2], si[ISFEW ? 512 : PIECE];  // the piece's keys, one beside each end
     const int lane = threadIdx.x % TPR, g = threadIdx.x / TPR;
     const int col = (blockIdx.y * TPR + lane) * 8;
     const int ncol = a.N - col;
-    const int64_t p0 = (int64_t)blockIdx.x * GB * a.tg;
-    const int64_t lo = p0 + (int64_t)g * a.tg, hi = lo + a.tg < a.T ? lo + a.tg : a.T;
-    const bool any = lo < a.T;
-    if (any) {
-        uint32_t cur = a.key[lo];
-        const bool from = lo > 0 && a.key[lo - 1] == cur;
+    const int P = GB * a.tg;
+    const int64_t p0 = (int64_t)blockIdx.x * P;
+    int n;  // tokens of the piece
+    if constexpr (ISFEW) {
+        __shared__ FewLds L;
+        n = few_sort(a, p0, P, sk, si, L);
+        if (threadIdx.x == 0) {
+            sk[0] = NO_KEY;
+            sk[1 + n] = NO_KEY;
+        }
+    } else {
+        n = a.T - p0 < P ? (int)(a.T - p0) : P;
+        for (int i = threadIdx.x; i < n; i += 256) {
+            const uint2 v = a.kv[p0 + i];
+            sk[1 + i] = v.x;
+            si[i] = v.y;
+        }
+        if (threadIdx.x == 0) {
+            sk[0] = p0 > 0 ? a.kv[p0 - 1].x : NO_KEY;
+            sk[1 + n] = p0 + n < a.T ? a.kv[p0 + n].x : NO_KEY;
+        }
+    }
+    __syncthreads();
+    float* part = a.part + (int64_t)blockIdx.x * (ISFEW ? (int64_t)a.V : 2) * a.Np;
+    auto whole = [&](uint32_t key, const float s[8]) {  // the sum of a run that lies in the piece
+        if constexpr (ISFEW) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) part[(int64_t)key * a.Np + col + i] = s[i];
+        } else {
+            emb_out<T>(a, key, col, s);
+        }
+    };
+    const int lo = g * a.tg, hi = lo + a.tg < n ? lo + a.tg : n;
+    if (lo < n) {
+        uint32_t cur = sk[1 + lo];
+        const bool from = sk[lo] == cur;
         bool inhead = from;  // the run being summed came from before the group
         float s[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) s[i] = 0.f;
-        for (int64_t t0 = lo; t0 < hi; t0 += U) {
-            uint32_t kk[U];
+        for (int t0 = lo; t0 < hi; t0 += U) {
             Chunk<T> d[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int64_t t = t0 + u < hi ? t0 + u : hi - 1;
-                kk[u] = a.key[t];
-                d[u] = ld8((const T*)a.dy + (int64_t)a.idx[t] * a.lddy + col, ncol);
-            }
+            for (int u = 0; u < U; ++u) d[u] = ld8((const T*)a.dy + (int64_t)si[t0 + u < hi ? t0 + u : hi - 1] * a.lddy + col, ncol);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (t0 + u >= hi) break;
-                if (kk[u] != cur) {
+                const uint32_t k = sk[1 + t0 + u];
+                if (k != cur) {
                     if (inhead) {
 #pragma unroll
                         for (int i = 0; i < 8; ++i) head[g][lane * 8 + i] = s[i];
                     } else if (ncol > 0) {
-                        emb_out<T>(a, cur, col, s);
+                        whole(cur, s);
                     }
                     inhead = false;
-                    cur = kk[u];
+                    cur = k;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) s[i] = 0.f;
                 }
@@ -377,7 +532,7 @@ template <class T, int TPR> __global__ __launch_bounds__(256) void k_emb_seg(Emb
                 for (int i = 0; i < 8; ++i) s[i] += d[u].get(i);
             }
         }
-        const bool on = hi < a.T && a.key[hi] == cur;
+        const bool on = sk[1 + hi] == cur;
         if (inhead) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) head[g][lane * 8 + i] = s[i];
@@ -385,58 +540,78 @@ template <class T, int TPR> __global__ __launch_bounds__(256) void k_emb_seg(Emb
 #pragma unroll
             for (int i = 0; i < 8; ++i) tail[g][lane * 8 + i] = s[i];
         } else if (ncol > 0) {
-            emb_out<T>(a, cur, col, s);
+            whole(cur, s);
         }
         if (lane == 0) {
-            first[g] = a.key[lo];
             last[g] = cur;
             hflag[g] = from ? 1 : 0;
             tflag[g] = on ? (inhead ? 2 : 1) : 0;
         }
     }
     __syncthreads();
-    if (g != 0 || ncol <= 0) return;
-    // the groups' open runs joined in order by the first group's lanes
+    if (lo >= n || ncol <= 0) return;
+    // a run over several groups is joined, in order, by the group where it begins
+    const int ng = (n + a.tg - 1) / a.tg;
     float c[8];
-    bool open = false, prev = false;
-    uint32_t ck = 0;
-    float* part = a.part + (int64_t)blockIdx.x * 2 * a.Np;
+    auto join = [&](int q) {  // adds the heads from group q on; whether the run ends in the piece
+        for (; q < ng; ++q) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = 0.f;
-    for (int q = 0; q < GB && p0 + (int64_t)q * a.tg < a.T; ++q) {
-        if (hflag[q]) {
-            if (q == 0) {
-                prev = true;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) c[i] = head[0][lane * 8 + i];
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) c[i] += head[q][lane * 8 + i];
-            }
-            open = true;
-            ck = first[q];
-            if (tflag[q] == 2) continue;  // the whole group is inside the run
-            if (prev) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) part[col + i] = c[i];
-            } else {
-                emb_out<T>(a, ck, col, c);
-            }
-            open = prev = false;
+            for (int i = 0; i < 8; ++i) c[i] += head[q][lane * 8 + i];
+            if (tflag[q] != 2) return true;
         }
-        if (tflag[q] == 1) {
-            open = true;
-            prev = false;
-            ck = last[q];
+        return false;
+    };
+    if (g == 0 && hflag[0]) {  // from the piece before (it may go on behind this one): the head partial
 #pragma unroll
-            for (int i = 0; i < 8; ++i) c[i] = tail[q][lane * 8 + i];
+        for (int i = 0; i < 8; ++i) c[i] = 0.f;
+        join(0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) part[col + i] = c[i];
+    }
+    if (tflag[g] == 1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = tail[g][lane * 8 + i];
+        if (join(g + 1)) {
+            whole(last[g], c);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) part[a.Np + col + i] = c[i];
         }
     }
-    if (open) {  // goes on in the next piece
-        float* o = part + (prev ? 0 : a.Np);
+}
+// few rows: row blockIdx.x, the pieces' partials in order (group g: pieces g, g + GB, ..)
+template <class T, int TPR> __global__ __launch_bounds__(256) void k_emb_few_join(EmbB a, int pieces) {
+    constexpr int GB = 256 / TPR, U = 4;
+    __shared__ float sh[GB][TPR * 8];
+    const int lane = threadIdx.x % TPR, g = threadIdx.x / TPR;
+    const int col = (blockIdx.y * TPR + lane) * 8;
+    const uint32_t v = blockIdx.x;
+    float s[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[col + i] = c[i];
-    }
+    for (int i = 0; i < 8; ++i) s[i] = 0.f;
+    if (col < a.N)
+        for (int j0 = g; j0 < pieces; j0 += GB * U) {
+            uint32_t has[U];
+            Chunk<float> h[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int j = j0 + u * GB < pieces ? j0 + u * GB : j0;
+                has[u] = j0 + u * GB < pieces ? a.cnt[(int64_t)j * a.V + v] : 0;
+                h[u] = Chunk<float>::load(a.part + ((int64_t)j * a.V + v) * a.Np + col);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s[i] += has[u] ? h[u].get(i) : 0.f;  // (a row it lacks: never written)
+        }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sh[g][lane * 8 + i] = s[i];
+    __syncthreads();
+    if (g != 0 || col >= a.N) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        for (int q = 1; q < GB; ++q) s[i] += sh[q][lane * 8 + i];
+    emb_out<T>(a, v, col, s);
 }
 // workgroup = the run that goes on behind piece blockIdx.x and begins in it (else nothing to do)
 template <class T, int TPR> __global__ __launch_bounds__(256) void k_emb_join(EmbB a, int pieces) {
@@ -445,19 +620,19 @@ template <class T, int TPR> __global__ __launch_bounds__(256) void k_emb_join(Em
     __shared__ int cnt;
     const int64_t P = (int64_t)GB * a.tg;
     const int64_t c = blockIdx.x, lo = c * P, hi = lo + P;  // (hi < T: the last piece has no workgroup)
-    const uint32_t key = a.key[hi];
-    if (key >= a.V || a.key[hi - 1] != key) return;
-    if (c > 0 && a.key[lo - 1] == key) return;  // begins in an earlier piece (the keys are sorted)
+    const uint32_t key = a.kv[hi].x;
+    if (key >= a.V || a.kv[hi - 1].x != key) return;
+    if (c > 0 && a.kv[lo - 1].x == key) return;  // begins in an earlier piece (the keys are sorted)
     if (threadIdx.x == 0) cnt = 0;
     __syncthreads();
     // pieces behind c that the run fills to their end and beyond
     for (int64_t j0 = c + 1; j0 < pieces; j0 += 256) {
         const int64_t j = j0 + threadIdx.x, e = (j + 1) * P;
-        const bool in = j < pieces && e < a.T && a.key[e] == key;
+        const bool in = j < pieces && e < a.T && a.kv[e].x == key;
         const uint64_t m = __ballot(in);
         if ((threadIdx.x & 63) == 0 && m) atomicAdd(&cnt, __popcll(m));
         const int64_t e1 = (j0 + 256) * P;  // the last of these pieces
-        if (e1 >= a.T || a.key[e1] != key) break;
+        if (e1 >= a.T || a.kv[e1].x != key) break;
     }
     __syncthreads();
     const int64_t end = c + 1 + cnt;  // the last piece of the run
@@ -467,10 +642,14 @@ template <class T, int TPR> __global__ __launch_bounds__(256) void k_emb_join(Em
 #pragma unroll
     for (int i = 0; i < 8; ++i) s[i] = 0.f;
     if (col < a.N)
-        for (int64_t j = c + 1 + g; j <= end; j += GB) {
-            const Chunk<float> h = Chunk<float>::load(a.part + j * 2 * a.Np + col);
+        for (int64_t j0 = c + 1 + g; j0 <= end; j0 += GB * 4) {
+            Chunk<float> h[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s[i] += h.get(i);
+            for (int u = 0; u < 4; ++u) h[u] = Chunk<float>::load(a.part + (j0 + u * GB <= end ? j0 + u * GB : j0) * 2 * a.Np + col);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s[i] += j0 + u * GB <= end ? h[u].get(i) : 0.f;
         }
 #pragma unroll
     for (int i = 0; i < 8; ++i) sh[g][lane * 8 + i] = s[i];
@@ -488,14 +667,6 @@ template <class T, int TPR> __global__ __launch_bounds__(256) void k_emb_join(Em
 // =======================================================================================
 // Host side
 // =======================================================================================
-// threads per row of the chunk-walking kernels
-static int ltpr_for(int64_t N) {
-    const int64_t nc = (N + 7) / 8;
-    int l = 0;
-    while (l < 8 && (int64_t(1) << l) < nc) ++l;
-    return l;
-}
-
 hipError_t norm_fwd(const mmvae_norm_args& a, hipStream_t st) {
     if (a.M == 0) return hipSuccess;
     return a.dtype == MMVAE_T_F32 ? norm_fwd_f32(a, st) : a.dtype == MMVAE_T_BF16 ? norm_fwd_bf16(a, st) : norm_fwd_f16(a, st);
@@ -507,11 +678,9 @@ hipError_t norm_bwd(const mmvae_norm_args& a, hipStream_t st) {
 hipError_t dropout(const mmvae_dropout_args& a, hipStream_t st) {
     if (a.M == 0 || a.N == 0) return hipSuccess;
     const DropKey k = drop_key(a.p, a.seed, a.step, a.row_offset, a.state);
-    const int l = ltpr_for(a.N), rpb = 256 >> l;
-    const int64_t g = std::min<int64_t>((a.M + rpb - 1) / rpb, 4096);
     return by_type(a.dtype, [&](auto ty) -> hipError_t {
         using T = decltype(ty);
-        return launch(k_dropout<T>, dim3((unsigned)g), dim3(256), st, a.M, a.N, (const T*)a.x, a.ldx, (T*)a.y, a.ldy, l, k);
+        return launch(k_dropout<T>, dim3((unsigned)walk_blocks(a.M, a.N)), dim3(256), st, a.M, (int)a.N, (const T*)a.x, a.ldx, (T*)a.y, a.ldy, k);
     });
 }
 
@@ -530,27 +699,33 @@ hipError_t emb_fwd(const mmvae_embedding_args& a, hipStream_t st) {
     p.y = a.y;
     p.scale = a.scale;
     p.i64 = a.ids64;
-    const int l = ltpr_for(a.N), rpb = 256 >> l;
-    const int64_t g = std::min<int64_t>((a.T + rpb - 1) / rpb, 4096);
     return by_type(a.dtype, [&](auto ty) -> hipError_t {
-        return launch(k_emb_fwd<decltype(ty)>, dim3((unsigned)g), dim3(256), st, p, l);
+        return launch(k_emb_fwd<decltype(ty)>, dim3((unsigned)walk_blocks(a.T, a.N)), dim3(256), st, p);
     });
 }
 
-// the gradient's plan, a function of (T, N) alone: tokens per group and pieces
+// the gradient's plan, a function of (T, N, V) alone: tokens per group and pieces
 struct EmbPlan {
+    bool few;
     int tpr, gb, tg, slices;
     int64_t pieces, tiles, Np;
-    int64_t o_key[2], o_idx[2], o_hist, o_part, bytes;
+    int64_t o_kv[2], o_hist, o_part, bytes;
 };
-static EmbPlan emb_plan(int64_t T, int64_t N) {
+static EmbPlan emb_plan(int64_t T, int64_t N, int64_t V) {
     EmbPlan q;
-    q.Np = (N + 7) / 8 * 8;
-    const int l = std::min(ltpr_for(N), 6);
-    q.tpr = std::max(8, 1 << l);
+    std::memset(&q, 0, sizeof(q));
+    const int64_t nc = (N + 7) / 8;
+    q.Np = nc * 8;
+    q.few = V <= FEW;
+    // lanes a row: 32, or 16 where 32 would leave over a fifth more of them idle (262144 x 128 bf16: 16 lanes
+    // 15.6 us, 32 23.1 us; 50001 x 517 f16: 16 lanes 25.1 us, 32 23.3 us, 64 22.9 us, 8 29.6 us)
+    auto lanes = [&](int64_t t) { return (nc + t - 1) / t * t; };
+    q.tpr = nc <= 8 ? 8 : 5 * lanes(32) > 6 * lanes(16) ? 16 : 32;
     q.gb = 256 / q.tpr;
-    q.slices = (int)((N + q.tpr * 8 - 1) / (q.tpr * 8));
-    q.tg = T > 32768 ? 32 : 8;
+    q.slices = (int)((nc + q.tpr - 1) / q.tpr);
+    // a group's tokens: 8 in one go of loads; more for long inputs, so that the partials stay few beside dy
+    q.tg = T > 32768 ? 16 : 8;
+    if (q.few && T > 32768) q.tg = 512 / q.gb;
     q.pieces = std::max<int64_t>(1, (T + (int64_t)q.gb * q.tg - 1) / ((int64_t)q.gb * q.tg));
     q.tiles = (T + RTILE - 1) / RTILE;
     int64_t o = 0;
@@ -559,76 +734,78 @@ static EmbPlan emb_plan(int64_t T, int64_t N) {
         o += (b + 255) / 256 * 256;
         return at;
     };
-    for (int i = 0; i < 2; ++i) {
-        q.o_key[i] = take(T * 4);
-        q.o_idx[i] = take(T * 4);
-    }
-    q.o_hist = take((q.tiles + 1) * 256 * 4);
-    q.o_part = take(q.pieces * 2 * q.Np * 4);
+    if (!q.few)
+        for (int i = 0; i < (T <= RONE ? 1 : 2); ++i) q.o_kv[i] = take(T * 8);
+    q.o_hist = take(q.few ? q.pieces * V * 4 : (q.tiles + 1) * 256 * 4);
+    q.o_part = take(q.pieces * (q.few ? V : 2) * q.Np * 4);
     q.bytes = o;
     return q;
 }
-int64_t emb_bwd_ws(int64_t T, int64_t N) { return emb_plan(T, N).bytes; }
+int64_t emb_bwd_ws(int64_t T, int64_t N, int64_t V) { return T == 0 || V == 0 ? 0 : emb_plan(T, N, V).bytes; }
 
 __global__ __launch_bounds__(1024) void k_emb_clear(void* out, int64_t out_bytes) {
-    fill_zero((uint32_t*)out, out_bytes / 4, (int64_t)blockIdx.x * 1024 + threadIdx.x, (int64_t)gridDim.x * 1024);
-    if (blockIdx.x == 0 && threadIdx.x == 0 && (out_bytes & 2)) ((uint16_t*)out)[out_bytes / 2 - 1] = 0;
+    fill_zero(out, out_bytes, (int64_t)blockIdx.x * 1024 + threadIdx.x, (int64_t)gridDim.x * 1024);
 }
 
 hipError_t emb_bwd(const mmvae_embedding_args& a, hipStream_t st) {
     const int64_t z = a.dtype == MMVAE_T_F32 ? 4 : 2, out_bytes = a.V * a.N * z;
     const int clear = (int)std::min<int64_t>((out_bytes / 4 + RTHR * 4 - 1) / (RTHR * 4) + 1, 1024);
-    if (a.T == 0) return out_bytes ? launch(k_emb_clear, dim3((unsigned)clear), dim3(1024), st, a.dtable, out_bytes) : hipSuccess;
-    const EmbPlan q = emb_plan(a.T, a.N);
+    if (out_bytes == 0) return hipSuccess;
+    if (a.T == 0) return launch(k_emb_clear, dim3((unsigned)clear), dim3(1024), st, a.dtable, out_bytes);
+    const EmbPlan q = emb_plan(a.T, a.N, a.V);
     char* ws = (char*)a.ws;
-    uint32_t* key[2] = {(uint32_t*)(ws + q.o_key[0]), (uint32_t*)(ws + q.o_key[1])};
-    uint32_t* idx[2] = {(uint32_t*)(ws + q.o_idx[0]), (uint32_t*)(ws + q.o_idx[1])};
+    uint2* kv[2] = {(uint2*)(ws + q.o_kv[0]), (uint2*)(ws + q.o_kv[1])};
     uint32_t* hist = (uint32_t*)(ws + q.o_hist);
     const uint32_t V = (uint32_t)a.V;
     int passes = 1;
     while (passes < 4 && (V >> (8 * passes)) != 0) ++passes;
     int cur = 0;
-    if (a.T <= RTILE) {
-        OPCHK(launch(k_emb_sort1, dim3((unsigned)(1 + clear)), dim3(RTHR), st, a.ids, a.ids64, (int)a.T, V, passes, key[0], idx[0],
-                     a.dtable, out_bytes));
-    } else {
+    if (!q.few && a.T <= RONE) {
+        OPCHK(launch(k_emb_sort1, dim3((unsigned)(1 + clear)), dim3(RTHR), st, a.ids, a.ids64, (int)a.T, V, passes, kv[0], a.dtable, out_bytes));
+    } else if (!q.few) {
         const int tiles = (int)q.tiles, scanned = tiles > RFUSE ? 1 : 0;
         for (int p = 0; p < passes; ++p) {
-            const uint32_t* ki = p ? key[cur] : nullptr;
-            const uint32_t* xi = p ? idx[cur] : nullptr;
+            const uint2* from = p ? kv[cur] : nullptr;
             const int nxt = p ? cur ^ 1 : 0;
-            OPCHK(launch(k_emb_hist, dim3((unsigned)(tiles + (p ? 0 : clear))), dim3(RTHR), st, a.ids, a.ids64, ki, a.T, V, 8 * p, tiles,
+            OPCHK(launch(k_emb_hist, dim3((unsigned)(tiles + (p ? 0 : clear))), dim3(RTHR), st, a.ids, a.ids64, from, a.T, V, 8 * p, tiles,
                          hist, a.dtable, out_bytes));
             if (scanned) OPCHK(launch(k_emb_scan, dim3(256), dim3(256), st, tiles, hist));
-            OPCHK(launch(k_emb_scatter, dim3((unsigned)tiles), dim3(RTHR), st, a.ids, a.ids64, ki, xi, a.T, V, 8 * p, tiles, scanned,
-                         (const uint32_t*)hist, key[nxt], idx[nxt]));
+            OPCHK(launch(k_emb_scatter, dim3((unsigned)tiles), dim3(RTHR), st, a.ids, a.ids64, from, a.T, V, 8 * p, tiles, scanned,
+                         (const uint32_t*)hist, kv[nxt]));
             cur = nxt;
         }
     }
     EmbB b;
+    std::memset(&b, 0, sizeof(b));
     b.T = a.T;
     b.N = (int)a.N;
     b.Np = q.Np;
     b.V = V;
-    b.key = key[cur];
-    b.idx = idx[cur];
+    b.kv = kv[cur];
+    b.ids = a.ids;
+    b.i64 = a.ids64;
     b.dy = a.dy;
     b.lddy = a.lddy;
     b.out = a.dtable;
     b.part = (float*)(ws + q.o_part);
+    b.cnt = hist;
     b.scale = a.scale;
     b.tg = q.tg;
     const dim3 grid((unsigned)q.pieces, (unsigned)q.slices), jgrid((unsigned)(q.pieces - 1), (unsigned)q.slices);
+    const dim3 fgrid((unsigned)a.V, (unsigned)q.slices);
     return by_type(a.dtype, [&](auto ty) -> hipError_t {
         using T = decltype(ty);
         auto go = [&](auto t) -> hipError_t {
-            OPCHK(launch(k_emb_seg<T, t.value>, grid, dim3(256), st, b));
+            if (q.few) {
+                OPCHK(launch(k_emb_seg<T, t.value, true>, grid, dim3(256), st, b));
+                return launch(k_emb_few_join<T, t.value>, fgrid, dim3(256), st, b, (int)q.pieces);
+            }
+            OPCHK(launch(k_emb_seg<T, t.value, false>, grid, dim3(256), st, b));
             return q.pieces > 1 ? launch(k_emb_join<T, t.value>, jgrid, dim3(256), st, b, (int)q.pieces) : hipSuccess;
         };
         if (q.tpr == 8) return go(I<8>{});
         if (q.tpr == 16) return go(I<16>{});
-        if (q.tpr == 32) return go(I<32>{});
-        return go(I<64>{});
+        return go(I<32>{});
     });
 }
 
@@ -658,6 +835,7 @@ const char* norm_check(const mmvae_norm_args& a, bool bwd) {
 }
 const char* dropout_check(const mmvae_dropout_args& a) {
     if (a.M < 0 || a.N < 0 || a.M > MAX_DIM || a.N > MAX_DIM) return "need 0 <= M, N < 2^31";
+    if (a.M > 0 && a.N > 0 && (a.N >= (1 << 24) || walk_blocks(a.M, a.N) > MAX_DIM)) return "need N < 2^24, and M N below 2^44";
     if (!type_ok(a.dtype)) return "types: f32, bf16 or f16";
     if (const char* m = drop_check(a.p)) return m;
     if (a.M > 0 && a.N > 0 && (!a.x || !a.y)) return "x or y is null";
@@ -668,6 +846,7 @@ const char* emb_check(const mmvae_embedding_args& a, bool bwd) {
     if (a.T < 0 || a.N < 1 || a.V < 0 || a.T > MAX_DIM || a.N >= (1 << 24) || a.V > MAX_DIM)
         return "need 0 <= T, V < 2^31 and 1 <= N < 2^24";
     if (!type_ok(a.dtype)) return "types: f32, bf16 or f16";
+    if (walk_blocks(a.T, a.N) > MAX_DIM) return "need T N below 2^44";
     if (a.T > 0 && !a.ids) return "ids is null";
     if (!bwd) {
         if (a.T > 0 && a.V > 0 && !a.table) return "table is null";
@@ -679,7 +858,9 @@ const char* emb_check(const mmvae_embedding_args& a, bool bwd) {
     if (a.V > 0 && !a.dtable) return "dtable is null";
     if (a.lddy < 0) return "dy's row stride is negative";
     if ((uintptr_t)a.dtable & 3) return "dtable must be 4-byte aligned";
-    if (a.T > 0 && (!a.ws || a.ws_bytes < emb_bwd_ws(a.T, a.N))) return "the workspace is below mmvae_embedding_bwd_ws(T, N) bytes";
+    if (emb_bwd_ws(a.T, a.N, a.V) > 0 && (!a.ws || a.ws_bytes < emb_bwd_ws(a.T, a.N, a.V)))
+        return "the workspace is below mmvae_embedding_bwd_ws(T, N, V) bytes";
+    if (((uintptr_t)a.ws & 15) != 0) return "the workspace must be 16-byte aligned";
     return nullptr;
 }
 
@@ -726,6 +907,6 @@ int mmvae_embedding_fwd(const mmvae_embedding_args* a) {
 int mmvae_embedding_bwd(const mmvae_embedding_args* a) {
     return op_call("embedding_bwd", a, a ? emb_check(*a, true) : "null arguments", emb_bwd);
 }
-int64_t mmvae_embedding_bwd_ws(int64_t T, int64_t N) { return T < 0 || N < 1 ? 0 : emb_bwd_ws(T, N); }
+int64_t mmvae_embedding_bwd_ws(int64_t T, int64_t N, int64_t V) { return T < 0 || N < 1 || V < 0 ? 0 : emb_bwd_ws(T, N, V); }
 
 }  // extern "C"

@@ -20,7 +20,7 @@ hipError_t norm_bwd_f16(const mmvae_norm_args& a, hipStream_t st);
 hipError_t dropout(const mmvae_dropout_args& a, hipStream_t st);
 hipError_t emb_fwd(const mmvae_embedding_args& a, hipStream_t st);
 hipError_t emb_bwd(const mmvae_embedding_args& a, hipStream_t st);
-int64_t emb_bwd_ws(int64_t T, int64_t N);
+int64_t emb_bwd_ws(int64_t T, int64_t N, int64_t V);
 const char* norm_check(const mmvae_norm_args& a, bool bwd);
 const char* dropout_check(const mmvae_dropout_args& a);
 const char* emb_check(const mmvae_embedding_args& a, bool bwd);

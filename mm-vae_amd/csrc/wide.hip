@@ -2344,7 +2344,7 @@ hipError_t wide_create(Engine* e) {
             if ((er = norm_bufs(L)) != hipSuccess) return er;
     if (e->cfg.n_labels > 0) {
         WA(w->Zl, Bp * K);
-        w->op_ws_bytes = std::max(w->op_ws_bytes, emb_bwd_ws(Bp, K));
+        w->op_ws_bytes = std::max(w->op_ws_bytes, emb_bwd_ws(Bp, K, e->cfg.n_labels));
     }
     if (w->op_ws_bytes > 0 && (er = hipMalloc(&w->op_ws, (size_t)w->op_ws_bytes)) != hipSuccess) return er;
 #undef WA

@@ -110,7 +110,7 @@ def lib():
         "mmvae_dropout": (ctypes.c_int, [ctypes.c_char_p]),
         "mmvae_embedding_fwd": (ctypes.c_int, [ctypes.c_char_p]),
         "mmvae_embedding_bwd": (ctypes.c_int, [ctypes.c_char_p]),
-        "mmvae_embedding_bwd_ws": (i64, [i64, i64]),
+        "mmvae_embedding_bwd_ws": (i64, [i64, i64, i64]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)

@@ -196,7 +196,7 @@ def embedding_backward(dy, ids, rows, scale=1.0):
     if not isinstance(rows, int) or rows < 0:
         _wrong("rows must be the table's row count")
     out = d2.new_empty((rows, N))
-    n = lib().mmvae_embedding_bwd_ws(T, N)
+    n = lib().mmvae_embedding_bwd_ws(T, N, rows)
     ws = d2.new_empty((n,), dtype=torch.uint8)
     dev = d2.get_device()
     rc = lib().mmvae_embedding_bwd(_EMB.pack(T, N, rows, i.data_ptr(), 0, 0, 0, 0, 0, 0, d2.data_ptr(), d2.stride(0), out.data_ptr(), ws.data_ptr(), n,

@@ -83,7 +83,7 @@ def test_norm_backward_refuses(kw):
 
 
 @pytest.mark.parametrize("kw", [dict(M=-1), dict(N=-1), dict(N=2 ** 31), dict(dtype=5), dict(p=-1.0), dict(p=2.0), dict(p=float("nan")), dict(x=0),
-                                dict(y=0), dict(ldx=-8), dict(ldy=7)])
+                                dict(y=0), dict(ldx=-8), dict(ldy=7), dict(N=1 << 24, ldx=1 << 24, ldy=1 << 24)])
 def test_dropout_refuses(kw):
     assert mmvae_amd.lib().mmvae_dropout(pack_drop(**kw)) == -1
 
@@ -95,7 +95,7 @@ def test_embedding_forward_refuses(kw):
 
 
 @pytest.mark.parametrize("kw", [dict(T=-1), dict(N=0), dict(V=-1), dict(dtype=3), dict(ids=0), dict(dy=0), dict(dtable=0), dict(dtable=4098), dict(lddy=-1),
-                                dict(ws=0), dict(ws_bytes=100)])
+                                dict(ws=0), dict(ws_bytes=100), dict(ws=4100), dict(V=1000, ws_bytes=100)])
 def test_embedding_backward_refuses(kw):
     assert mmvae_amd.lib().mmvae_embedding_bwd(pack_emb(**kw)) == -1
 
@@ -109,15 +109,16 @@ def test_null_arguments_refused():
 def test_workspace_sizes_grow_with_the_call():
     L = mmvae_amd.lib()
     assert L.mmvae_layer_norm_bwd_ws(-1, 8) == 0 and L.mmvae_layer_norm_bwd_ws(4, 0) == 0
-    assert L.mmvae_embedding_bwd_ws(-1, 8) == 0 and L.mmvae_embedding_bwd_ws(4, 0) == 0
+    assert L.mmvae_embedding_bwd_ws(-1, 8, 5) == 0 and L.mmvae_embedding_bwd_ws(4, 0, 5) == 0 and L.mmvae_embedding_bwd_ws(4, 8, -1) == 0
     for N in (1, 7, 64, 100, 1000, 20000, 32768, 32769, 100000):
         for M in (0, 1, 2, 100, 4096):  # few rows: one workgroup, no partial sums
             n = L.mmvae_layer_norm_bwd_ws(M, N)
             assert n >= 2 * 2 * 4 * N or (n == 0 and M <= (256 if N <= 1024 else 1)) or (N > 32768 and n >= 2 * 4 * N)
         assert L.mmvae_layer_norm_bwd_ws(4096, N) > 0
-    # two sorted copies of the tokens (id, position), and a partial head and tail of a piece at least
+    # the sorted tokens (id, place), and a partial head and tail of a piece at least
     for T in (1, 4096, 4097, 600000):
-        assert L.mmvae_embedding_bwd_ws(T, 33) >= 16 * T + 2 * 4 * 40
+        assert L.mmvae_embedding_bwd_ws(T, 33, 1000) >= 8 * T + 2 * 4 * 40
+        assert L.mmvae_embedding_bwd_ws(T, 33, 7) >= 7 * 4 * 40  # few rows: a partial of each
 
 
 @pytest.mark.parametrize("call", [
