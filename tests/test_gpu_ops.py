@@ -34,9 +34,9 @@ def close(got, want, bound, what):
 
 def c_norm(name, x, w, b, y=0, ldy=0, mean=0, rstd=0, dy=0, lddy=0, dx=0, lddx=0, dw=0, db=0, ws=0, ws_bytes=0):
     """The C entry itself, for outputs where the caller wants them."""
-    rc = getattr(mmvae_amd.lib(), name)(ops._NORM.pack(
+    rc = getattr(mmvae_amd.lib(), name)(ops.NORM_ARGS.pack(
         x.shape[0], x.shape[1], x.data_ptr(), x.stride(0), w.data_ptr(), b.data_ptr(), y, ldy, mean, rstd, dy, lddy, dx, lddx, dw, db, ws, ws_bytes,
-        0.0, 0, 0, 0, 0, torch.cuda.current_stream().cuda_stream, 0, ops._TYPE[x.dtype], 0, 1e-5, 0, 0))
+        0.0, 0, 0, 0, 0, torch.cuda.current_stream().cuda_stream, 0, {F32: 0, BF16: 1, F16: 2}[x.dtype], 0, 1e-5, 0, 0))
     assert rc == 0
 
 

@@ -21,20 +21,20 @@ def pack_norm(**kw):
     v = dict(M=4, N=8, x=4096, ldx=8, w=0, b=0, y=4096, ldy=8, mean=4096, rstd=4096, dy=4096, lddy=8, dx=4096, lddx=8, dw=4096, db=4096,
              ws=4096, ws_bytes=1 << 30, p=0.0, seed=1, step=0, row_offset=0, state=0, stream=0, device=0, dtype=0, wtype=0, eps=1e-5, relu=0, reserved=0)
     v.update(kw)
-    return ops._NORM.pack(*v.values())
+    return ops.NORM_ARGS.pack(*v.values())
 
 
 def pack_drop(**kw):
     v = dict(M=4, N=8, x=4096, ldx=8, y=4096, ldy=8, p=0.5, seed=1, step=0, row_offset=0, state=0, stream=0, device=0, dtype=0)
     v.update(kw)
-    return ops._DROP.pack(*v.values())
+    return ops.DROPOUT_ARGS.pack(*v.values())
 
 
 def pack_emb(**kw):
     v = dict(T=4, N=8, V=3, ids=4096, table=4096, ldt=8, add=0, ldadd=8, y=4096, ldy=8, dy=4096, lddy=8, dtable=4096, ws=4096,
              ws_bytes=1 << 30, stream=0, device=0, dtype=0, ids64=1, scale=1.0)
     v.update(kw)
-    return ops._EMB.pack(*v.values())
+    return ops.EMBEDDING_ARGS.pack(*v.values())
 
 
 def test_packed_structs_match_the_header(tmp_path):
@@ -54,7 +54,7 @@ def test_packed_structs_match_the_header(tmp_path):
     c.write_text("#include <stddef.h>\n#include <stdio.h>\n#include \"mmvae_capi.h\"\nint main(void) {%s return 0; }\n" % "\n".join(lines))
     subprocess.run(["gcc", "-I", INCLUDE, str(c), "-o", str(tmp_path / "o")], check=True)
     out = subprocess.run([str(tmp_path / "o")], check=True, capture_output=True, text=True).stdout.splitlines()
-    for line, st in zip(out, (ops._NORM, ops._DROP, ops._EMB)):
+    for line, st in zip(out, (ops.NORM_ARGS, ops.DROPOUT_ARGS, ops.EMBEDDING_ARGS)):
         size, *offs = [int(v) for v in line.split()[1:]]
         assert size >= st.size and size - st.size < 8, line
         want, at = [], 0
