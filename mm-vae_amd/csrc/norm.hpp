@@ -30,12 +30,24 @@ struct NormP {
 // u = xh w + b, as forward and backward both compute it (the ReLU's side must be the same)
 MMVAE_DEV float ln_u(float x, float mean, float rstd, float w, float b) { return __builtin_fmaf((x - mean) * rstd, w, b); }
 
-// A thread's weights stay with it over its rows: in registers, or for rows of more than 8192 columns
-// (BLK = 1024) in LDS, where they leave the registers to the row.  Biases that do not fit there too
-// (N > 20,480) are read with every row.
-template <int BLK> struct LnHold {
-    static constexpr bool LDS = BLK == 1024;
+// How a thread keeps its row and weights, by the registers that a wave has (256 at 512 threads, 128 at
+// 1024; with fewer threads a row other rows' waves hide the loads too):
+//   HOLD  the weights in registers over all rows, else in LDS (16 V of w and b forward, 8 V of w backward);
+//   PRE   the next row's loads in flight under this row's sums;
+//   AGAIN (backward) x and dy read in both phases, where they do not fit beside the 16 V column sums.
+// ROOM: what is left beside temporaries, as the compiler uses them (no variant that is launched spills
+// more than a few registers).
+template <class T, int VPT, int BLK, bool MASK, bool EVEN> struct LnKeep {
+    static constexpr int X = (int)sizeof(T) * 2;  // registers of a chunk
+    static constexpr int ROOM = (BLK >= 1024 ? 128 : 256) - 66 - (MASK ? 10 : 0) - (EVEN ? 0 : 14);
+    static constexpr int B = 16 + (MASK ? 12 : 0);  // a chunk's column sums (and masks)
+    static constexpr bool F_HOLD = (16 + X) * VPT <= ROOM;
+    static constexpr bool F_PRE = ((F_HOLD ? 16 : 0) + 2 * X) * VPT <= ROOM;
+    static constexpr bool B_AGAIN = (B + 2 * X) * VPT > ROOM;
+    static constexpr bool B_PRE = !B_AGAIN && (B + 4 * X) * VPT <= ROOM;
+    static constexpr bool B_HOLD = !B_AGAIN && (B + (B_PRE ? 4 : 2) * X + 8) * VPT <= ROOM;
 };
+
 static constexpr int LN_LDS = 163840;  // bytes of LDS of a CU
 
 // a pointer into LDS that the compiler takes for a new one: what is read there is read again (with every
@@ -50,7 +62,8 @@ MMVAE_DEV float* lds_anew(float* l) {
 template <class T, int TPR, int VPT, int BLK, bool MASK, bool EVEN>
 __global__ __launch_bounds__(BLK) void k_ln_fwd(NormP a) {
     constexpr int RPB = BLK / TPR;
-    constexpr bool HOLD = !LnHold<BLK>::LDS;
+    typedef LnKeep<T, VPT, BLK, MASK, EVEN> Keep;
+    constexpr bool HOLD = Keep::F_HOLD, PRE = Keep::F_PRE;
     extern __shared__ float4 dyn_lds[];
     float* lw = reinterpret_cast<float*>(dyn_lds);
     __shared__ float red[2][BLK / 64];
@@ -69,16 +82,24 @@ __global__ __launch_bounds__(BLK) void k_ln_fwd(NormP a) {
             if (a.b_lds) lds_put8(lw + slots * 8, slots, c, hb[0]);
         }
     }
-    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.M; r0 += (int64_t)gridDim.x * RPB) {
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    Chunk<T> xc[VPT], xn[PRE ? VPT : 1];
+    auto fetch = [&](int64_t r, Chunk<T>* x) {
+        const T* xr = (const T*)a.x + (r < a.M ? r : 0) * a.ldx;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) x[j] = ld_row<EVEN>(xr, (j * TPR + lane) * 8, N);
+    };
+    if constexpr (PRE) fetch((int64_t)blockIdx.x * RPB + grp, xn);
+    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.M; r0 += step) {
         const int64_t row = r0 + grp;
         const bool ok = row < a.M;
-        const T* xr = (const T*)a.x + (ok ? row : 0) * a.ldx;
-        Chunk<T> xc[VPT];
         float s = 0.f;
+        if constexpr (PRE) {
 #pragma unroll
-        for (int j = 0; j < VPT; ++j) {
-            const int col = (j * TPR + lane) * 8;
-            xc[j] = ld_row<EVEN>(xr, col, N);
+            for (int j = 0; j < VPT; ++j) xc[j] = xn[j];
+            if (r0 + step < a.M) fetch(row + step, xn);
+        } else {
+            fetch(row, xc);
         }
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
@@ -149,7 +170,8 @@ __global__ __launch_bounds__(BLK) void k_ln_fwd(NormP a) {
 template <class T, int TPR, int VPT, int BLK, bool MASK, bool EVEN>
 __global__ __launch_bounds__(BLK, BLK / 256) void k_ln_bwd(NormP a) {
     constexpr int RPB = BLK / TPR;
-    constexpr bool HOLD = !LnHold<BLK>::LDS || TPR <= 64, AGAIN = VPT >= 3 && (MASK || VPT == 4 || sizeof(T) == 4);
+    typedef LnKeep<T, VPT, BLK, MASK, EVEN> Keep;
+    constexpr bool HOLD = Keep::B_HOLD, AGAIN = Keep::B_AGAIN, PRE = Keep::B_PRE;
     extern __shared__ float4 dyn_lds[];
     float* lw = reinterpret_cast<float*>(dyn_lds);
     __shared__ float red[2][BLK / 64];
@@ -169,33 +191,49 @@ __global__ __launch_bounds__(BLK, BLK / 256) void k_ln_bwd(NormP a) {
     for (int j = 0; j < VPT; ++j)
 #pragma unroll
         for (int i = 0; i < 8; ++i) aw[j][i] = ab[j][i] = 0.f;
-    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.M; r0 += (int64_t)gridDim.x * RPB) {
-        const int64_t row = r0 + grp;
-        const bool ok = row < a.M;
-        const T* xr = (const T*)a.x + (ok ? row : 0) * a.ldx;
-        const T* dr = (const T*)a.dy + (ok ? row : 0) * a.lddy;
-        const float mean = ok ? a.mean[row] : 0.f, rstd = ok ? a.rstd[row] : 0.f;
-        // a row's x and dy, dy without what dropout and ReLU take away: du = ds dc.  (AGAIN: too many for the
-        // registers beside the sums; each phase reads them, the second with the first's bits)
-        Chunk<T> xc[AGAIN ? 1 : VPT], dc[AGAIN ? 1 : VPT];
-        uint32_t bits[VPT];
-        auto read = [&](int j) {
-            const int col = (j * TPR + lane) * 8;
-            Chunk<T>&x = xc[AGAIN ? 0 : j], &d = dc[AGAIN ? 0 : j];
-            x = ld_row<EVEN>(xr, col, N);
-            d = ld_row<EVEN>(dr, col, N);
-            if ((EVEN && col >= N) || !ok) d = Chunk<T>{};  // adds nothing
-        };
+    // a row's x and dy, dy without what dropout and ReLU take away: du = ds dc.  (AGAIN: each phase reads
+    // them, the second with the first's bits)
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    Chunk<T> xc[AGAIN ? 1 : VPT], dc[AGAIN ? 1 : VPT], xn[PRE ? VPT : 1], dn[PRE ? VPT : 1];
+    uint32_t bits[VPT];
+    float mean = 0.f, rstd = 0.f, mean_n = 0.f, rstd_n = 0.f;
+    auto read = [&](int64_t r, int j, Chunk<T>& x, Chunk<T>& d) {
+        const int col = (j * TPR + lane) * 8;
+        const bool ok = r < a.M;
+        x = ld_row<EVEN>((const T*)a.x + (ok ? r : 0) * a.ldx, col, N);
+        d = ld_row<EVEN>((const T*)a.dy + (ok ? r : 0) * a.lddy, col, N);
+    };
+    auto fetch = [&](int64_t r, Chunk<T>* x, Chunk<T>* d, float& m, float& s) {
+        m = r < a.M ? a.mean[r] : 0.f;
+        s = r < a.M ? a.rstd[r] : 0.f;
         if constexpr (!AGAIN) {
 #pragma unroll
-            for (int j = 0; j < VPT; ++j) read(j);
+            for (int j = 0; j < VPT; ++j) read(r, j, x[j], d[j]);
+        }
+    };
+    if constexpr (PRE) fetch((int64_t)blockIdx.x * RPB + grp, xn, dn, mean_n, rstd_n);
+    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.M; r0 += step) {
+        const int64_t row = r0 + grp;
+        const bool ok = row < a.M;
+        if constexpr (PRE) {
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                xc[j] = xn[j];
+                dc[j] = dn[j];
+            }
+            mean = mean_n;
+            rstd = rstd_n;
+            if (r0 + step < a.M) fetch(row + step, xn, dn, mean_n, rstd_n);
+        } else {
+            fetch(row, xc, dc, mean, rstd);
         }
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-            if constexpr (AGAIN) read(j);
             const int c = j * TPR + lane, col = c * 8, n = N - col;
             Chunk<T>&x = xc[AGAIN ? 0 : j], &dd = dc[AGAIN ? 0 : j];
+            if constexpr (AGAIN) read(row, j, x, dd);
+            if ((EVEN && col >= N) || !ok) dd = Chunk<T>{};  // adds nothing
             float w[8], b[8];
             if constexpr (HOLD) {
 #pragma unroll
@@ -253,7 +291,7 @@ __global__ __launch_bounds__(BLK, BLK / 256) void k_ln_bwd(NormP a) {
                     const int col = (j * TPR + lane) * 8, n = N - col;
                     if (n <= 0) continue;
                     if constexpr (AGAIN) {
-                        read(j);
+                        read(row, j, xc[0], dc[0]);
                         bool on[8];
 #pragma unroll
                         for (int i = 0; i < 8; ++i) on[i] = (bits[j] >> i) & 1;
@@ -499,12 +537,14 @@ template <class F> inline hipError_t by_width(int N, F&& f) {
     if (nc <= 256) return f(I<256>{}, I<1>{}, I<256>{});
     if (nc <= 512) return f(I<256>{}, I<2>{}, I<256>{});
     if (nc <= 1024) return f(I<512>{}, I<2>{}, I<512>{});
-    if (nc <= 2048) return f(I<1024>{}, I<2>{}, I<1024>{});
-    if (nc <= 3072) return f(I<1024>{}, I<3>{}, I<1024>{});
-    return f(I<1024>{}, I<4>{}, I<1024>{});
+    if (nc <= 1536) return f(I<512>{}, I<3>{}, I<512>{});
+    if (nc <= 2048) return f(I<512>{}, I<4>{}, I<512>{});
+    if (nc <= 2560) return f(I<512>{}, I<5>{}, I<512>{});
+    if (nc <= 3072) return f(I<512>{}, I<6>{}, I<512>{});
+    return f(I<512>{}, I<8>{}, I<512>{});
 }
 // a backward of few rows in one workgroup of 1024, which writes dw and db itself: rows it may have
-constexpr int ONE_ROUNDS = 2;
+constexpr int ONE_ROUNDS = 2, LONG_PARTS = 128;
 inline bool norm_one(int64_t M, int64_t N) {
     const int nc = (int)((std::min<int64_t>(N, LONG_N) + 7) / 8);
     int tpr = 8;
@@ -549,7 +589,7 @@ inline int norm_rpb(int64_t N) {  // rows a workgroup holds at once
 // workgroups of the backward = rows of partial weight sums
 inline int64_t norm_parts(int64_t M, int64_t N) {
     if (norm_one(M, N)) return 1;
-    if (N > LONG_N) return std::min<int64_t>(M, 32);
+    if (N > LONG_N) return std::min<int64_t>(M, LONG_PARTS);
     const int64_t need = (M + norm_rpb(N) - 1) / norm_rpb(N);
     return std::min<int64_t>(need, N > 8192 ? 256 : 512);
 }
@@ -573,12 +613,12 @@ template <class T> hipError_t norm_fwd_t(const mmvae_norm_args& a, hipStream_t s
     return by_width(p.N, [&](auto t, auto v, auto b) -> hipError_t {
         constexpr int RPB = b.value / t.value;
         const int64_t g = std::min<int64_t>((a.M + RPB - 1) / RPB, 256 * (2048 / b.value));
-        size_t lds = 0;
-        if (LnHold<b.value>::LDS) {
-            p.b_lds = 2 * p.Np * 4 <= LN_LDS - 256;  // (beside the waves' sums)
-            lds = (p.b_lds ? 2 : 1) * (size_t)p.Np * 4;
-        }
         return by_flags(p, [&](auto m, auto e) {
+            size_t lds = 0;
+            if (!LnKeep<T, v.value, b.value, m.value, e.value>::F_HOLD) {
+                p.b_lds = 2 * p.Np * 4 <= LN_LDS - 256;  // (beside the waves' sums)
+                lds = (p.b_lds ? 2 : 1) * (size_t)p.Np * 4;
+            }
             return launch_lds(lds, k_ln_fwd<T, t.value, v.value, b.value, m.value, e.value>, dim3((unsigned)g), dim3(b.value), st, p);
         });
     });
@@ -594,16 +634,18 @@ template <class T> hipError_t norm_bwd_t(const mmvae_norm_args& a, hipStream_t s
     p.part = wg && !one ? (float*)a.ws : nullptr;
     p.dw = a.dw;
     p.db = a.db;
-    const int64_t G = norm_parts(a.M, a.N);
+    // (with masks the sums of more than 20,480 columns do not stay in the registers: 228 bytes a lane spilled)
+    const bool sweeps = a.N > LONG_N || (!one && a.N > 20480 && (p.relu || p.drop.thr));
+    const int64_t G = sweeps ? std::min<int64_t>(a.M, LONG_PARTS) : norm_parts(a.M, a.N);
     if (a.M > 0 && (a.dx || wg)) {
-        if (a.N > LONG_N) {
+        if (sweeps) {
             if (wg)  // (first: dx may overwrite dy or x)
                 OPCHK(launch(k_ln_cols<T>, dim3((unsigned)((p.Np / 8 + 255) / 256), (unsigned)G), dim3(256), st, p));
             if (a.dx) OPCHK(launch(k_ln_bwd_long<T>, dim3((unsigned)std::min<int64_t>(a.M, 512)), dim3(1024), st, p));
         } else {
             auto go = [&](auto t, auto v, auto b) -> hipError_t {
-                const size_t lds = LnHold<b.value>::LDS && t.value > 64 ? (size_t)p.Np * 4 : 0;
                 return by_flags(p, [&](auto m, auto e) {
+                    const size_t lds = LnKeep<T, v.value, b.value, m.value, e.value>::B_HOLD ? 0 : (size_t)p.Np * 4;
                     return launch_lds(lds, k_ln_bwd<T, t.value, v.value, b.value, m.value, e.value>, dim3((unsigned)G), dim3(b.value), st, p);
                 });
             };

@@ -233,7 +233,9 @@ MMVAE_DEV void drop_state(DropKey& k) {
 // half shifted up; p = 1, thr = 65536, keeps none)
 MMVAE_DEV void keep8(const DropKey& k, int64_t row, int chunk, bool kept[8]) {
     const uint64_t r = (uint64_t)(k.row0 + row);
-    uint32_t c[4] = {(uint32_t)chunk, (uint32_t)r, (uint32_t)k.step, (uint32_t)((uint64_t)k.step >> 32) ^ (uint32_t)(r >> 32)};
+    uint32_t ch = (uint32_t)chunk;
+    asm volatile("" : "+v"(ch));  // (a chunk's first products, the same for every row, are not worth their registers)
+    uint32_t c[4] = {ch, (uint32_t)r, (uint32_t)k.step, (uint32_t)((uint64_t)k.step >> 32) ^ (uint32_t)(r >> 32)};
     philox4x32_10(c, k.k0, k.k1);
     const uint32_t t = k.thr << 16;
     const bool some = k.thr < 65536;
