@@ -27,8 +27,25 @@ struct NormP {
     DropKey drop;
 };
 
-// u = xh w + b, as forward and backward both compute it (the ReLU's side must be the same)
-MMVAE_DEV float ln_u(float x, float mean, float rstd, float w, float b) { return __builtin_fmaf((x - mean) * rstd, w, b); }
+// A row's statistics, and xh and u = xh w + b as forward and backward both compute them (the ReLU's side
+// must be the same).  f32: xh from the difference, exact near the mean; 16-bit values carry 2^-9 and more
+// themselves: one fma.  w and b come multiplied by the dropout factor (a ReLU commutes with it).
+template <class T> struct RowStat {
+    float mean, rstd, nm;
+    MMVAE_DEV void set(float m, float r) {
+        mean = m;
+        rstd = r;
+        nm = -m * r;
+    }
+    MMVAE_DEV float xh(float x) const { return sizeof(T) == 4 ? (x - mean) * rstd : __builtin_fmaf(x, rstd, nm); }
+    MMVAE_DEV float u(float x, float w, float b) const { return __builtin_fmaf(xh(x), w, b); }
+};
+// 8 weights times the factor
+template <class T> MMVAE_DEV void ldws(const void* w, bool f32, int col, int n, float none, float s, float v[8]) {
+    ldw<T>(w, f32, col, n, none, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= s;
+}
 
 // How a thread keeps its row and weights, by the registers that a wave has (256 at 512 threads, 128 at
 // 1024; with fewer threads a row other rows' waves hide the loads too):
@@ -69,14 +86,14 @@ __global__ __launch_bounds__(BLK) void k_ln_fwd(NormP a) {
     __shared__ float red[2][BLK / 64];
     const int lane = threadIdx.x % TPR, grp = threadIdx.x / TPR;
     const int N = a.N, slots = (N + 7) / 8;
-    const float inv = 1.f / (float)N;
+    const float inv = 1.f / (float)N, sc = MASK && a.drop.thr ? a.drop.s : 1.f;
     if (MASK) drop_state(a.drop);
     float hw[HOLD ? VPT : 1][8], hb[HOLD ? VPT : 1][8];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
         const int c = j * TPR + lane, col = c * 8;
-        ldw<T>(a.w, a.wf32, col, N - col, 1.f, hw[HOLD ? j : 0]);
-        if (HOLD || a.b_lds) ldw<T>(a.b, a.wf32, col, N - col, 0.f, hb[HOLD ? j : 0]);
+        ldws<T>(a.w, a.wf32, col, N - col, 1.f, sc, hw[HOLD ? j : 0]);
+        if (HOLD || a.b_lds) ldws<T>(a.b, a.wf32, col, N - col, 0.f, sc, hb[HOLD ? j : 0]);
         if (!HOLD && c < slots) {
             lds_put8(lw, slots, c, hw[0]);
             if (a.b_lds) lds_put8(lw + slots * 8, slots, c, hb[0]);
@@ -121,7 +138,8 @@ __global__ __launch_bounds__(BLK) void k_ln_fwd(NormP a) {
             }
             q += !EVEN || n > 0 ? t : 0.f;
         }
-        const float rstd = 1.f / sqrtf(row_sum<TPR>(q, red[1]) * inv + a.eps);
+        RowStat<T> st;
+        st.set(mean, 1.f / sqrtf(row_sum<TPR>(q, red[1]) * inv + a.eps));
         if (ok) {
             T* yr = (T*)a.y + row * a.ldy;
             const float* rw = HOLD ? lw : lds_anew(lw);
@@ -133,12 +151,12 @@ __global__ __launch_bounds__(BLK) void k_ln_fwd(NormP a) {
                 if constexpr (!HOLD) {
                     lds_get8(rw, slots, c, w);
                     if (a.b_lds) lds_get8(rw + slots * 8, slots, c, b);
-                    else ldw<T>(a.b, a.wf32, col, n, 0.f, b);
+                    else ldws<T>(a.b, a.wf32, col, n, 0.f, sc, b);
                 }
                 float u[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    u[i] = ln_u(xc[j].get(i), mean, rstd, HOLD ? hw[HOLD ? j : 0][i] : w[i], HOLD ? hb[HOLD ? j : 0][i] : b[i]);
+                    u[i] = st.u(xc[j].get(i), HOLD ? hw[HOLD ? j : 0][i] : w[i], HOLD ? hb[HOLD ? j : 0][i] : b[i]);
                 if (MASK && a.relu) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) u[i] = u[i] > 0.f || u[i] != u[i] ? u[i] : 0.f;  // (a NaN stays one)
@@ -147,7 +165,7 @@ __global__ __launch_bounds__(BLK) void k_ln_fwd(NormP a) {
                     bool kept[8];
                     keep8(a.drop, row, c, kept);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) u[i] = kept[i] ? u[i] * a.drop.s : 0.f;
+                    for (int i = 0; i < 8; ++i) u[i] = kept[i] ? u[i] : 0.f;
                 }
                 Chunk<T> yc;
 #pragma unroll
@@ -157,7 +175,7 @@ __global__ __launch_bounds__(BLK) void k_ln_fwd(NormP a) {
             }
             if (lane == 0) {
                 if (a.mean) a.mean[row] = mean;
-                if (a.rstd) a.rstd[row] = rstd;
+                if (a.rstd) a.rstd[row] = st.rstd;
             }
         }
         if constexpr (TPR > 64) __syncthreads();  // the next row's sums reuse `red`
@@ -165,7 +183,7 @@ __global__ __launch_bounds__(BLK) void k_ln_fwd(NormP a) {
 }
 
 // backward: du = dy m [u > 0], g = du w, dx = rstd (g - mean(g) - xh mean(g xh)); the workgroup's
-// sums of du xh and du over its rows (fixed order: a thread's rows, then the row groups) -> part, or
+// sums of du xh and du over its rows (of the unscaled du: times the dropout factor once, at the end) (fixed order: a thread's rows, then the row groups) -> part, or
 // with one workgroup straight into dw / db.  Elements behind a row's end are loaded as 0 and add 0.
 template <class T, int TPR, int VPT, int BLK, bool MASK, bool EVEN>
 __global__ __launch_bounds__(BLK, BLK / 256) void k_ln_bwd(NormP a) {
@@ -183,7 +201,7 @@ __global__ __launch_bounds__(BLK, BLK / 256) void k_ln_bwd(NormP a) {
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
         const int c = j * TPR + lane, col = c * 8;
-        ldw<T>(a.w, a.wf32, col, N - col, 1.f, hw[HOLD ? j : 0]);
+        ldws<T>(a.w, a.wf32, col, N - col, 1.f, ds, hw[HOLD ? j : 0]);
         if (!HOLD && c < slots) lds_put8(lw, slots, c, hw[0]);
     }
     float aw[VPT][8], ab[VPT][8];
@@ -191,7 +209,7 @@ __global__ __launch_bounds__(BLK, BLK / 256) void k_ln_bwd(NormP a) {
     for (int j = 0; j < VPT; ++j)
 #pragma unroll
         for (int i = 0; i < 8; ++i) aw[j][i] = ab[j][i] = 0.f;
-    // a row's x and dy, dy without what dropout and ReLU take away: du = ds dc.  (AGAIN: each phase reads
+    // a row's x and dy, dy without what dropout and ReLU take away: du = ds dc, g = dc (ds w).  (AGAIN: each phase reads
     // them, the second with the first's bits)
     const int64_t step = (int64_t)gridDim.x * RPB;
     Chunk<T> xc[AGAIN ? 1 : VPT], dc[AGAIN ? 1 : VPT], xn[PRE ? VPT : 1], dn[PRE ? VPT : 1];
@@ -227,6 +245,8 @@ __global__ __launch_bounds__(BLK, BLK / 256) void k_ln_bwd(NormP a) {
         } else {
             fetch(row, xc, dc, mean, rstd);
         }
+        RowStat<T> st;
+        st.set(mean, rstd);
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
@@ -245,9 +265,9 @@ __global__ __launch_bounds__(BLK, BLK / 256) void k_ln_bwd(NormP a) {
                 bool on[8] = {true, true, true, true, true, true, true, true};
                 if (a.drop.thr) keep8(a.drop, row, c, on);
                 if (a.relu) {
-                    ldw<T>(a.b, a.wf32, col, n, 0.f, b);
+                    ldws<T>(a.b, a.wf32, col, n, 0.f, ds, b);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) on[i] = on[i] && ln_u(x.get(i), mean, rstd, w[i], b[i]) > 0.f;
+                    for (int i = 0; i < 8; ++i) on[i] = on[i] && st.u(x.get(i), w[i], b[i]) > 0.f;
                 }
                 dd.keep(on);
                 if constexpr (AGAIN) {
@@ -258,9 +278,7 @@ __global__ __launch_bounds__(BLK, BLK / 256) void k_ln_bwd(NormP a) {
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float xh = (x.get(i) - mean) * rstd;
-                const float d = MASK ? dd.get(i) * ds : dd.get(i);
-                const float dxh = d * xh;
+                const float d = dd.get(i), dxh = d * st.xh(x.get(i));
                 aw[j][i] += dxh;
                 ab[j][i] += d;
                 s1 = __builtin_fmaf(d, w[i], s1);
@@ -284,6 +302,8 @@ __global__ __launch_bounds__(BLK, BLK / 256) void k_ln_bwd(NormP a) {
                 }
             }
             const float c1 = row_sum<TPR>(s1, red[0]) * inv, c2 = row_sum<TPR>(s2, red[1]) * inv;
+            // dx = d (w rstd) + x A + B: the row's part, - rstd (c1 + xh c2), is linear in x
+            const float A = -rstd * rstd * c2, B = -rstd * c1 - mean * A;
             if (ok) {
                 T* yr = (T*)a.y + row * a.ldy;
 #pragma unroll
@@ -308,9 +328,8 @@ __global__ __launch_bounds__(BLK, BLK / 256) void k_ln_bwd(NormP a) {
                     Chunk<T> o;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const float xh = (x.get(i) - mean) * rstd;
-                        const float d = MASK ? dd.get(i) * ds : dd.get(i);
-                        o.set(i, rstd * (__builtin_fmaf(d, w[i], -c1) - xh * c2));
+                        const float r = sizeof(T) == 4 ? __builtin_fmaf(x.get(i) - mean, A, -rstd * c1) : __builtin_fmaf(x.get(i), A, B);
+                        o.set(i, __builtin_fmaf(dd.get(i), w[i] * rstd, r));
                     }
                     if constexpr (EVEN) o.store(yr + col);
                     else st8(yr + col, n, o);
@@ -323,6 +342,7 @@ __global__ __launch_bounds__(BLK, BLK / 256) void k_ln_bwd(NormP a) {
     if (!a.part && !a.dw && !a.db) return;
     // a column's sum: into the partials, or (one workgroup) rounded into the gradients
     auto put = [&](int h, int c, float v) {
+        if (MASK) v *= ds;
         if (a.part) {
             a.part[((int64_t)blockIdx.x * 2 + h) * a.Np + c] = v;
         } else if (c < N) {
@@ -399,7 +419,7 @@ static constexpr int LONG_N = 32768;
 template <class T> __global__ __launch_bounds__(1024) void k_ln_fwd_long(NormP a) {
     __shared__ float red[2][16];
     const int N = a.N;
-    const float inv = 1.f / (float)N;
+    const float inv = 1.f / (float)N, sc = a.drop.thr ? a.drop.s : 1.f;
     drop_state(a.drop);
     for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
         const T* xr = (const T*)a.x + row * a.ldx;
@@ -424,49 +444,51 @@ template <class T> __global__ __launch_bounds__(1024) void k_ln_fwd_long(NormP a
             }
             q += t;
         }
-        const float rstd = 1.f / sqrtf(row_sum<1024>(q, red[1]) * inv + a.eps);
+        RowStat<T> st;
+        st.set(mean, 1.f / sqrtf(row_sum<1024>(q, red[1]) * inv + a.eps));
         T* yr = (T*)a.y + row * a.ldy;
         for (int64_t col = threadIdx.x * 8; col < N; col += 8192) {
             const int n = (int)(N - col);
             const Chunk<T> c = ld8(xr + col, n);
             float w[8], b[8];
             bool kept[8];
-            ldw<T>(a.w, a.wf32, (int)col, n, 1.f, w);
-            ldw<T>(a.b, a.wf32, (int)col, n, 0.f, b);
+            ldws<T>(a.w, a.wf32, (int)col, n, 1.f, sc, w);
+            ldws<T>(a.b, a.wf32, (int)col, n, 0.f, sc, b);
             if (a.drop.thr) keep8(a.drop, row, (int)(col >> 3), kept);
             Chunk<T> yc;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                float u = ln_u(c.get(i), mean, rstd, w[i], b[i]);
+                float u = st.u(c.get(i), w[i], b[i]);
                 if (a.relu) u = u > 0.f || u != u ? u : 0.f;
-                if (a.drop.thr) u = kept[i] ? u * a.drop.s : 0.f;
+                if (a.drop.thr) u = kept[i] ? u : 0.f;
                 yc.set(i, u);
             }
             st8(yr + col, n, yc);
         }
         if (threadIdx.x == 0) {
             if (a.mean) a.mean[row] = mean;
-            if (a.rstd) a.rstd[row] = rstd;
+            if (a.rstd) a.rstd[row] = st.rstd;
         }
         __syncthreads();
     }
 }
-// one chunk's du and xh
+// one chunk's dy without what dropout and ReLU take away, xh, and the weights times the dropout factor
 template <class T>
-MMVAE_DEV void ln_du(const NormP& a, int64_t row, int64_t col, float mean, float rstd, float w[8], float du[8], float xh[8]) {
+MMVAE_DEV void ln_du(const NormP& a, int64_t row, int64_t col, const RowStat<T>& st, float w[8], float du[8], float xh[8]) {
     const int n = (int)(a.N - col);
     const Chunk<T> xc = ld8((const T*)a.x + row * a.ldx + col, n), dc = ld8((const T*)a.dy + row * a.lddy + col, n);
+    const float sc = a.drop.thr ? a.drop.s : 1.f;
     float b[8];
     bool kept[8];
-    ldw<T>(a.w, a.wf32, (int)col, n, 1.f, w);
-    if (a.relu) ldw<T>(a.b, a.wf32, (int)col, n, 0.f, b);
+    ldws<T>(a.w, a.wf32, (int)col, n, 1.f, sc, w);
+    if (a.relu) ldws<T>(a.b, a.wf32, (int)col, n, 0.f, sc, b);
     if (a.drop.thr) keep8(a.drop, row, (int)(col >> 3), kept);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        xh[i] = i < n ? (xc.get(i) - mean) * rstd : 0.f;
+        xh[i] = i < n ? st.xh(xc.get(i)) : 0.f;
         float d = dc.get(i);
-        if (a.drop.thr) d = kept[i] ? d * a.drop.s : 0.f;
-        if (a.relu) d = ln_u(xc.get(i), mean, rstd, w[i], b[i]) > 0.f ? d : 0.f;
+        if (a.drop.thr) d = kept[i] ? d : 0.f;
+        if (a.relu) d = st.u(xc.get(i), w[i], b[i]) > 0.f ? d : 0.f;
         du[i] = i < n ? d : 0.f;
     }
 }
@@ -475,10 +497,11 @@ template <class T> __global__ __launch_bounds__(1024) void k_ln_bwd_long(NormP a
     const float inv = 1.f / (float)a.N;
     drop_state(a.drop);
     for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
-        const float mean = a.mean[row], rstd = a.rstd[row];
+        RowStat<T> st;
+        st.set(a.mean[row], a.rstd[row]);
         float s1 = 0.f, s2 = 0.f, w[8], du[8], xh[8];
         for (int64_t col = threadIdx.x * 8; col < a.N; col += 8192) {
-            ln_du<T>(a, row, col, mean, rstd, w, du, xh);
+            ln_du<T>(a, row, col, st, w, du, xh);
             float t1 = 0.f, t2 = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -491,10 +514,10 @@ template <class T> __global__ __launch_bounds__(1024) void k_ln_bwd_long(NormP a
         const float c1 = row_sum<1024>(s1, red[0]) * inv, c2 = row_sum<1024>(s2, red[1]) * inv;
         T* yr = (T*)a.y + row * a.ldy;
         for (int64_t col = threadIdx.x * 8; col < a.N; col += 8192) {
-            ln_du<T>(a, row, col, mean, rstd, w, du, xh);
+            ln_du<T>(a, row, col, st, w, du, xh);
             Chunk<T> o;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o.set(i, rstd * (__builtin_fmaf(du[i], w[i], -c1) - xh[i] * c2));
+            for (int i = 0; i < 8; ++i) o.set(i, st.rstd * (__builtin_fmaf(du[i], w[i], -c1) - xh[i] * c2));
             st8(yr + col, (int)(a.N - col), o);
         }
         __syncthreads();
@@ -507,7 +530,9 @@ template <class T> __global__ __launch_bounds__(256) void k_ln_cols(NormP a) {
     drop_state(a.drop);
     float aw[8] = {}, ab[8] = {}, w[8], du[8], xh[8];
     for (int64_t row = blockIdx.y; row < a.M; row += gridDim.y) {
-        ln_du<T>(a, row, col, a.mean[row], a.rstd[row], w, du, xh);
+        RowStat<T> st;
+        st.set(a.mean[row], a.rstd[row]);
+        ln_du<T>(a, row, col, st, w, du, xh);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             aw[i] += du[i] * xh[i];
@@ -517,8 +542,8 @@ template <class T> __global__ __launch_bounds__(256) void k_ln_cols(NormP a) {
     float* pw = a.part + (int64_t)blockIdx.y * 2 * a.Np;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        pw[col + i] = aw[i];
-        pw[a.Np + col + i] = ab[i];
+        pw[col + i] = a.drop.thr ? aw[i] * a.drop.s : aw[i];
+        pw[a.Np + col + i] = a.drop.thr ? ab[i] * a.drop.s : ab[i];
     }
 }
 
@@ -591,7 +616,7 @@ inline int64_t norm_parts(int64_t M, int64_t N) {
     if (norm_one(M, N)) return 1;
     if (N > LONG_N) return std::min<int64_t>(M, LONG_PARTS);
     const int64_t need = (M + norm_rpb(N) - 1) / norm_rpb(N);
-    return std::min<int64_t>(need, N > 8192 ? 256 : 512);
+    return std::min<int64_t>(need, N > 4096 ? 256 : 512);
 }
 inline int64_t norm_ws_bytes(int64_t M, int64_t N) {
     if (norm_one(M, N)) return 0;

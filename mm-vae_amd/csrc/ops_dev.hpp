@@ -235,8 +235,19 @@ MMVAE_DEV void keep8(const DropKey& k, int64_t row, int chunk, bool kept[8]) {
     const uint64_t r = (uint64_t)(k.row0 + row);
     uint32_t ch = (uint32_t)chunk;
     asm volatile("" : "+v"(ch));  // (a chunk's first products, the same for every row, are not worth their registers)
-    uint32_t c[4] = {ch, (uint32_t)r, (uint32_t)k.step, (uint32_t)((uint64_t)k.step >> 32) ^ (uint32_t)(r >> 32)};
-    philox4x32_10(c, k.k0, k.k1);
+    uint32_t c0 = ch, c1 = (uint32_t)r, c2 = (uint32_t)k.step, c3 = (uint32_t)((uint64_t)k.step >> 32) ^ (uint32_t)(r >> 32);
+    uint32_t k0 = k.k0, k1 = k.k1;
+#pragma unroll
+    for (int i = 0; i < 10; ++i) {  // (common.hpp's rounds, each three-way xor in one instruction)
+        const uint64_t p0 = (uint64_t)0xD2511F53u * c0, p1 = (uint64_t)0xCD9E8D57u * c2;
+        c0 = __builtin_amdgcn_bitop3_b32((uint32_t)(p1 >> 32), c1, k0, 0x96);
+        c2 = __builtin_amdgcn_bitop3_b32((uint32_t)(p0 >> 32), c3, k1, 0x96);
+        c1 = (uint32_t)p1;
+        c3 = (uint32_t)p0;
+        k0 += 0x9E3779B9u;
+        k1 += 0xBB67AE85u;
+    }
+    const uint32_t c[4] = {c0, c1, c2, c3};
     const uint32_t t = k.thr << 16;
     const bool some = k.thr < 65536;
 #pragma unroll
