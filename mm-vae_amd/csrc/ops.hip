@@ -812,6 +812,8 @@ hipError_t emb_bwd(const mmvae_embedding_args& a, hipStream_t st) {
 // ---- argument checks: null, or what is wrong -------------------------------------------------
 static bool type_ok(int t) { return t == MMVAE_T_F32 || t == MMVAE_T_BF16 || t == MMVAE_T_F16; }
 static constexpr int64_t MAX_DIM = (int64_t(1) << 31) - 65536;  // rows, widths, tokens and table rows
+static constexpr int64_t MAX_WALK = (int64_t(1) << 24) - 1;     // workgroups of 256 threads: a grid has below 2^32 threads
+static bool aligned(const void* p, int type) { return ((uintptr_t)p & (type == MMVAE_T_F32 ? 3 : 1)) == 0; }
 static bool ld_ok(int64_t ld, int64_t N, int64_t M) { return M <= 1 || ld >= N; }  // an output's rows may not overlap
 static const char* drop_check(double p) { return p >= 0. && p <= 1. ? nullptr : "p must be in [0, 1]"; }
 
@@ -823,6 +825,13 @@ const char* norm_check(const mmvae_norm_args& a, bool bwd) {
     if (const char* m = drop_check(a.p)) return m;
     if (a.ldx < 0 || a.lddy < 0) return "row strides must be >= 0";
     if (a.M > 0 && !a.x) return "x is null";
+    for (const void* p : {a.x, (const void*)a.y, a.dy, (const void*)a.dx})
+        if (!aligned(p, a.dtype)) return "x, y, dy and dx must be aligned to their type";
+    for (const void* p : {a.w, a.b, (const void*)a.dw, (const void*)a.db})
+        if (!aligned(p, a.wtype)) return "w, b, dw and db must be aligned to their type";
+    for (const void* p : {(const void*)a.mean, (const void*)a.rstd, (const void*)a.ws})
+        if (!aligned(p, MMVAE_T_F32)) return "mean, rstd and the workspace must be 4-byte aligned";
+    if (((uintptr_t)a.state & 7) != 0) return "state must be 8-byte aligned";
     if (!bwd) {
         if (a.M > 0 && !a.y) return "y is null";
         if (!ld_ok(a.ldy, a.N, a.M)) return "y's row stride is below N";
@@ -835,8 +844,9 @@ const char* norm_check(const mmvae_norm_args& a, bool bwd) {
 }
 const char* dropout_check(const mmvae_dropout_args& a) {
     if (a.M < 0 || a.N < 0 || a.M > MAX_DIM || a.N > MAX_DIM) return "need 0 <= M, N < 2^31";
-    if (a.M > 0 && a.N > 0 && (a.N >= (1 << 24) || walk_blocks(a.M, a.N) > MAX_DIM)) return "need N < 2^24, and M N below 2^44";
+    if (a.M > 0 && a.N > 0 && (a.N >= (1 << 24) || walk_blocks(a.M, a.N) > MAX_WALK)) return "need N < 2^24, and M N below 2^37";
     if (!type_ok(a.dtype)) return "types: f32, bf16 or f16";
+    if (!aligned(a.x, a.dtype) || !aligned(a.y, a.dtype) || ((uintptr_t)a.state & 7) != 0) return "x, y and state must be aligned to their types";
     if (const char* m = drop_check(a.p)) return m;
     if (a.M > 0 && a.N > 0 && (!a.x || !a.y)) return "x or y is null";
     if (a.ldx < 0 || !ld_ok(a.ldy, a.N, a.M)) return "x's row stride is negative or y's below N";
@@ -846,7 +856,10 @@ const char* emb_check(const mmvae_embedding_args& a, bool bwd) {
     if (a.T < 0 || a.N < 1 || a.V < 0 || a.T > MAX_DIM || a.N >= (1 << 24) || a.V > MAX_DIM)
         return "need 0 <= T, V < 2^31 and 1 <= N < 2^24";
     if (!type_ok(a.dtype)) return "types: f32, bf16 or f16";
-    if (walk_blocks(a.T, a.N) > MAX_DIM) return "need T N below 2^44";
+    if (walk_blocks(a.T, a.N) > MAX_WALK) return "need T N below 2^37";
+    for (const void* p : {a.table, a.add, (const void*)a.y, a.dy})
+        if (!aligned(p, a.dtype)) return "table, add, y and dy must be aligned to their type";
+    if (((uintptr_t)a.ids & (a.ids64 ? 7 : 3)) != 0) return "ids must be aligned to their type";
     if (a.T > 0 && !a.ids) return "ids is null";
     if (!bwd) {
         if (a.T > 0 && a.V > 0 && !a.table) return "table is null";

@@ -47,8 +47,12 @@ struct Rows {
         if (d == 0 || t.size(-1) == 0) wrong(std::string(name) + " needs a last dimension of at least 1");
         device = t.get_device();
         const at::Tensor* q = &t;
+        if (t.is_neg()) {  // (a lazily negated view)
+            copy = t.resolve_neg();
+            q = &copy;
+        }
         if (d != 2) {
-            copy = t.reshape({-1, t.size(-1)});
+            copy = q->reshape({-1, t.size(-1)});
             q = &copy;
         }
         if (q->stride(1) != 1 && q->size(1) > 1) {
@@ -78,7 +82,7 @@ struct Weights {
             wrong(std::string(name) + " must be a tensor of [" + std::to_string(x.N) + "] on x's device");
         const int c = type_code(t.scalar_type());
         if (c < 0 || (c != x.dtype && c != MMVAE_T_F32)) wrong(std::string(name) + ": x's type or float32");
-        if (!t.is_contiguous()) wrong(std::string(name) + " must be contiguous");
+        if (!t.is_contiguous() || t.is_neg()) wrong(std::string(name) + " must be contiguous");
         if (type >= 0 && type != c) wrong("weight and bias must have one type");
         type = c;
         st = t.scalar_type();

@@ -80,8 +80,8 @@ def check_norm(x, dy, w, b, relu=False, p=0.0, seed=0, step=0, row_offset=0, eps
 
 
 SIZES = [(1, 1), (3, 2), (5, 7), (2, 8), (33, 9), (100, 48), (64, 64), (17, 65), (70, 128), (31, 130), (9, 256), (11, 257), (5, 512), (6, 513),
-         (7, 1001), (3, 1024), (3, 1025), (2, 2048), (3, 2049), (2, 4096), (2, 4097), (3, 8192), (2, 8200), (2, 16384), (2, 16392), (3, 20000),
-         (2, 24577), (1, 30000), (2, 32768), (2, 32769), (3, 40003)]
+         (7, 1001), (3, 1024), (3, 1025), (2, 2048), (3, 2049), (2, 4096), (2, 4097), (3, 8192), (2, 8200), (2, 12288), (2, 12296), (2, 16384), (2, 16392), (2, 20480),
+         (3, 20000), (2, 20481), (2, 24576), (2, 24577), (1, 30000), (2, 32768), (2, 32769), (3, 40003)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -91,7 +91,8 @@ def test_norm_sizes(M, N, dtype):
 
 
 @pytest.mark.parametrize("relu,p", [(True, 0.0), (False, 0.3), (True, 0.3)])
-@pytest.mark.parametrize("M,N", [(5, 7), (100, 48), (31, 130), (6, 513), (7, 1001), (3, 2049), (2, 8200), (2, 20001), (2, 40003)])
+@pytest.mark.parametrize("M,N", [(5, 7), (100, 48), (31, 130), (6, 513), (7, 1001), (3, 2049), (2, 8200), (2, 12296), (2, 16400), (2, 20001),
+                                 (3, 20488), (1, 25000), (3, 30001), (2, 40003)])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_norm_relu_dropout(M, N, dtype, relu, p):
     check_norm(*make(M, N, dtype), relu=relu, p=p, seed=2 ** 40 + 99, step=2 ** 33 + 5, row_offset=1000)
@@ -126,6 +127,8 @@ def test_norm_other_layouts():
     assert y3[0].shape == (4, 16, 96) and y3[1].shape == (4, 16) and torch.equal(y3[0].view(64, 96), a)
     buf = torch.randn(64 * 96 + 1, device=DEV).to(BF16)
     check_norm(buf[1:].view(64, 96), dy.to(BF16), w, b)
+    z = torch.complex(x, x).conj().imag  # lazily negated
+    assert z.is_neg() and torch.equal(ops.layer_norm_forward(z, w, b)[0], ops.layer_norm_forward(-x, w, b)[0])
     v = ops.layer_norm_forward(x[0], w, b)
     assert v[0].shape == (96,) and torch.equal(v[0], a[0])
 
@@ -133,6 +136,20 @@ def test_norm_other_layouts():
 @pytest.mark.parametrize("M,N", [(4096, 128), (5000, 48), (20000, 9), (1500, 1024), (700, 20000)])
 def test_norm_many_rows(M, N):
     check_norm(*make(M, N, F32), p=0.1, seed=5)
+    check_norm(*make(M, N, BF16))
+
+
+@pytest.mark.parametrize("p", [1.0, 0.99, 1e-7])
+def test_norm_dropout_of_all_and_none(p):
+    x, dy, w, b = make(60, 70, F32)
+    y, dx, dw, db = check_norm(x, dy, w, b, p=p, seed=4, relu=True)
+    if p == 1.0:
+        assert not y.any() and not dx.any() and not dw.any() and not db.any()
+        x[3, 3] = float("inf")  # (its row is dropped whole)
+        y, m, r = ops.layer_norm_forward(x, w, b, p=p, seed=4)
+        assert not y.any()
+    if p == 1e-7:  # rounds to no dropout
+        assert torch.equal(y, ops.layer_norm_forward(x, w, b, relu=True)[0])
 
 
 def test_norm_offset_rows():

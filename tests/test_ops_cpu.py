@@ -66,10 +66,10 @@ def test_packed_structs_match_the_header(tmp_path):
 
 
 NORM_BAD = [dict(M=-1), dict(N=0), dict(M=2 ** 31), dict(N=2 ** 31), dict(dtype=3), dict(wtype=1), dict(dtype=1, wtype=2), dict(eps=-1e-6),
-            dict(eps=float("nan")), dict(eps=float("inf")), dict(p=-0.1), dict(p=1.1), dict(p=float("nan")), dict(x=0), dict(ldx=-1)]
+            dict(eps=float("nan")), dict(eps=float("inf")), dict(p=-0.1), dict(p=1.1), dict(p=float("nan")), dict(x=0), dict(ldx=-1), dict(x=4098), dict(w=4097, dtype=1, wtype=1), dict(state=4100)]
 
 
-@pytest.mark.parametrize("kw", NORM_BAD + [dict(y=0), dict(ldy=7)])
+@pytest.mark.parametrize("kw", NORM_BAD + [dict(y=0), dict(ldy=7), dict(y=4099, dtype=2), dict(mean=4098)])
 def test_norm_forward_refuses(kw):
     L = mmvae_amd.lib()
     assert L.mmvae_layer_norm_fwd(pack_norm(**kw)) == -1
@@ -83,13 +83,15 @@ def test_norm_backward_refuses(kw):
 
 
 @pytest.mark.parametrize("kw", [dict(M=-1), dict(N=-1), dict(N=2 ** 31), dict(dtype=5), dict(p=-1.0), dict(p=2.0), dict(p=float("nan")), dict(x=0),
-                                dict(y=0), dict(ldx=-8), dict(ldy=7), dict(N=1 << 24, ldx=1 << 24, ldy=1 << 24)])
+                                dict(y=0), dict(ldx=-8), dict(ldy=7), dict(N=1 << 24, ldx=1 << 24, ldy=1 << 24), dict(x=4097, dtype=1),
+                                dict(M=1 << 20, N=1 << 18, ldy=1 << 18)])
 def test_dropout_refuses(kw):
     assert mmvae_amd.lib().mmvae_dropout(pack_drop(**kw)) == -1
 
 
 @pytest.mark.parametrize("kw", [dict(T=-1), dict(N=0), dict(N=1 << 24), dict(V=-1), dict(V=2 ** 31), dict(T=2 ** 31), dict(dtype=-1), dict(ids=0),
-                                dict(table=0), dict(y=0), dict(ldt=-1), dict(ldadd=-1), dict(ldy=7)])
+                                dict(table=0), dict(y=0), dict(ldt=-1), dict(ldadd=-1), dict(ldy=7), dict(ids=4100), dict(table=4098),
+                                dict(T=1 << 20, N=1 << 18, ldy=1 << 18)])
 def test_embedding_forward_refuses(kw):
     assert mmvae_amd.lib().mmvae_embedding_fwd(pack_emb(**kw)) == -1
 
