@@ -132,9 +132,9 @@ static constexpr int RFUSE = 256;   // up to so many tiles a scatter workgroup s
 // tokens w 64 KPT + k 64 + lane).  wh[w][d]: first the wave's counts, then the count of d in earlier waves.
 struct RadixLds {
     uint32_t wh[RTHR / 64][256];
-    uint32_t tot[256];   // the tile's count of each digit
-    uint32_t base[256];  // exclusive sums of tot
-    uint32_t ws[4];
+    uint32_t tot[2][256];   // the tile's count of each digit; all tiles'
+    uint32_t base[2][256];  // exclusive sums of the two
+    uint32_t ws[8];
 };
 template <int RKPT> MMVAE_DEV void radix_rank(const uint32_t dig[RKPT], const bool val[RKPT], uint32_t rank[RKPT], RadixLds& L) {
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -142,25 +142,27 @@ template <int RKPT> MMVAE_DEV void radix_rank(const uint32_t dig[RKPT], const bo
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < RKPT; ++k) {
-        uint64_t m = __ballot(val[k]);
+        const uint32_t old = val[k] ? L.wh[w][dig[k]] : 0;  // (comes while the lanes of the same digit are found)
+        const uint64_t valid = __ballot(val[k]);
+        uint32_t m0 = (uint32_t)valid, m1 = (uint32_t)(valid >> 32);
 #pragma unroll
         for (int b = 0; b < 8; ++b) {
-            const bool bit = (dig[k] >> b) & 1;
-            const uint64_t bal = __ballot(bit);
-            m &= bit ? bal : ~bal;
+            const uint32_t bit = (uint32_t)((int32_t)(dig[k] << (31 - b)) >> 31);  // 0 or all ones
+            const uint64_t bal = __ballot(bit != 0);
+            m0 &= ~((uint32_t)bal ^ bit);
+            m1 &= ~((uint32_t)(bal >> 32) ^ bit);
         }
-        const uint32_t lt = __popcll(m & ((uint64_t(1) << lane) - 1));
-        const uint32_t old = val[k] ? L.wh[w][dig[k]] : 0;
+        const uint32_t lt = __builtin_amdgcn_mbcnt_hi(m1, __builtin_amdgcn_mbcnt_lo(m0, 0));
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        if (val[k] && lt == 0) L.wh[w][dig[k]] = old + __popcll(m);
+        if (val[k] && lt == 0) L.wh[w][dig[k]] = old + __popc(m0) + __popc(m1);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
         rank[k] = old + lt;
     }
     __syncthreads();
-    uint32_t t = 0;
     if (threadIdx.x < 256) {
+        uint32_t t = 0;
         uint32_t c[RTHR / 64];
 #pragma unroll
         for (int q = 0; q < RTHR / 64; ++q) c[q] = L.wh[q][threadIdx.x];
@@ -169,27 +171,28 @@ template <int RKPT> MMVAE_DEV void radix_rank(const uint32_t dig[RKPT], const bo
             L.wh[q][threadIdx.x] = t;
             t += c[q];
         }
-        L.tot[threadIdx.x] = t;
+        L.tot[0][threadIdx.x] = t;
     }
     __syncthreads();
 }
-// base[d] = sum of src[e] over e < d (256 digits, waves 0 .. 3)
-MMVAE_DEV void digit_scan(const uint32_t* src, RadixLds& L) {
+// base[k][d] = sum of tot[k][e] over e < d (waves 0 .. 3 the first, 4 .. 7 the second)
+MMVAE_DEV void digit_scan(RadixLds& L) {
+    const int k = threadIdx.x >> 8, d = threadIdx.x & 255;
     uint32_t own = 0, v = 0;
-    if (threadIdx.x < 256) {
-        own = v = src[threadIdx.x];
+    if (k < 2) {
+        own = v = L.tot[k][d];
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const uint32_t u = __shfl_up(v, o, 64);
-            if ((int)(threadIdx.x & 63) >= o) v += u;
+            if ((d & 63) >= o) v += u;
         }
-        if ((threadIdx.x & 63) == 63) L.ws[threadIdx.x >> 6] = v;
+        if ((d & 63) == 63) L.ws[threadIdx.x >> 6] = v;
     }
     __syncthreads();
-    if (threadIdx.x < 256) {
+    if (k < 2) {
         uint32_t b = v - own;
-        for (int q = 0; q < (int)(threadIdx.x >> 6); ++q) b += L.ws[q];
-        L.base[threadIdx.x] = b;
+        for (int q = 0; q < (d >> 6); ++q) b += L.ws[4 * k + q];
+        L.base[k][d] = b;
     }
     __syncthreads();
 }
@@ -232,10 +235,10 @@ __global__ __launch_bounds__(RTHR) void k_emb_sort1(const void* ids, int i64, in
 #pragma unroll
         for (int k = 0; k < KPT; ++k) dig[k] = (kk[k] >> (8 * p)) & 255;
         radix_rank<KPT>(dig, val, rank, L);
-        digit_scan(L.tot, L);
+        digit_scan(L);
 #pragma unroll
         for (int k = 0; k < KPT; ++k)
-            if (val[k]) sh[L.base[dig[k]] + L.wh[w][dig[k]] + rank[k]] = make_uint2(kk[k], ii[k]);
+            if (val[k]) sh[L.base[0][dig[k]] + L.wh[w][dig[k]] + rank[k]] = make_uint2(kk[k], ii[k]);
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < KPT; ++k) {
@@ -253,8 +256,8 @@ __global__ __launch_bounds__(RTHR) void k_emb_sort1(const void* ids, int i64, in
     }
 }
 
-// digit counts of each tile: hist[tile][256]; kv null: the first pass, from the ids.  Workgroups past
-// the tiles (first pass) clear the gradient.
+// digit counts of each tile, two 16-bit ones a word (digits d and d + 128): hist[tile][128]; kv null: the
+// first pass, from the ids.  Workgroups past the tiles (first pass) clear the gradient.
 __global__ __launch_bounds__(RTHR) void k_emb_hist(const void* ids, int i64, const uint2* kv, int64_t T, uint32_t V, int shift, int tiles,
                                                    uint32_t* hist, void* out, int64_t out_bytes) {
     if ((int)blockIdx.x >= tiles) {
@@ -271,16 +274,16 @@ __global__ __launch_bounds__(RTHR) void k_emb_hist(const void* ids, int i64, con
         if (t < T) atomicAdd(&h[((kv ? kv[t].x : emb_key(ids, i64, t, V)) >> shift) & 255], 1u);
     }
     __syncthreads();
-    if (threadIdx.x < 256) hist[(int64_t)blockIdx.x * 256 + threadIdx.x] = h[threadIdx.x];
+    if (threadIdx.x < 128) hist[(int64_t)blockIdx.x * 128 + threadIdx.x] = h[threadIdx.x] | h[threadIdx.x + 128] << 16;
 }
-// many tiles: hist[.][d] -> the count of d in earlier tiles, hist[tiles][d] its total (workgroup = digit)
-__global__ __launch_bounds__(256) void k_emb_scan(int tiles, uint32_t* hist) {
+// many tiles: before[tile][d] = the count of d in earlier tiles, before[tiles][d] its total (workgroup = digit)
+__global__ __launch_bounds__(256) void k_emb_scan(int tiles, const uint32_t* hist, uint32_t* before) {
     __shared__ uint32_t ws[4];
     const int d = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     uint32_t carry = 0;
     for (int b0 = 0; b0 < tiles; b0 += 256) {
         const int b = b0 + threadIdx.x;
-        const uint32_t own = b < tiles ? hist[(int64_t)b * 256 + d] : 0;
+        const uint32_t w2 = b < tiles ? hist[(int64_t)b * 128 + (d & 127)] : 0, own = d < 128 ? w2 & 0xffff : w2 >> 16;
         uint32_t v = own;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -289,25 +292,25 @@ __global__ __launch_bounds__(256) void k_emb_scan(int tiles, uint32_t* hist) {
         }
         if (lane == 63) ws[w] = v;
         __syncthreads();
-        uint32_t before = carry, all = 0;
+        uint32_t first = carry, all = 0;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            if (q < w) before += ws[q];
+            if (q < w) first += ws[q];
             all += ws[q];
         }
-        if (b < tiles) hist[(int64_t)b * 256 + d] = before + v - own;
+        if (b < tiles) before[(int64_t)b * 256 + d] = first + v - own;
         carry += all;
         __syncthreads();
     }
-    if (threadIdx.x == 0) hist[(int64_t)tiles * 256 + d] = carry;
+    if (threadIdx.x == 0) before[(int64_t)tiles * 256 + d] = carry;
 }
 // one pass: a tile's tokens, sorted by the digit in LDS first (so that a digit's tokens leave together),
 // to their places
 __global__ __launch_bounds__(RTHR) void k_emb_scatter(const void* ids, int i64, const uint2* kv, int64_t T, uint32_t V, int shift, int tiles,
-                                                      int scanned, const uint32_t* hist, uint2* kv2) {
+                                                      const uint32_t* hist, const uint32_t* before, uint2* kv2) {
     constexpr int KPT = RTILE / RTHR;
     __shared__ RadixLds L;
-    __shared__ uint32_t pre[4][256], all[4][256];
+    __shared__ uint32_t pre[8][256], all[8][256];
     __shared__ uint2 sh[RTILE];
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int64_t t0 = (int64_t)blockIdx.x * RTILE;
@@ -322,49 +325,60 @@ __global__ __launch_bounds__(RTHR) void k_emb_scatter(const void* ids, int i64, 
         kk[k] = v.x;
         ii[k] = v.y;
     }
-    {  // the digits' totals and their counts in earlier tiles
-        const int d = threadIdx.x & 255, q = threadIdx.x >> 8;
-        uint32_t p = 0, t = 0;
-        if (scanned) {
+    {  // the digits' totals and their counts in earlier tiles (eight groups of threads, two digits a thread)
+        const int d = threadIdx.x & 127, q = threadIdx.x >> 7;
+        uint32_t p0 = 0, p1 = 0, a0 = 0, a1 = 0;
+        if (before) {
             if (q == 0) {
-                p = hist[(int64_t)blockIdx.x * 256 + d];
-                t = hist[(int64_t)tiles * 256 + d];
+                p0 = before[(int64_t)blockIdx.x * 256 + d];
+                p1 = before[(int64_t)blockIdx.x * 256 + d + 128];
+                a0 = before[(int64_t)tiles * 256 + d];
+                a1 = before[(int64_t)tiles * 256 + d + 128];
             }
         } else {
-            for (int b0 = q; b0 < tiles; b0 += 64) {  // 16 loads in flight
+            for (int b0 = q; b0 < tiles; b0 += 128) {  // 16 loads in flight
                 uint32_t v[16];
 #pragma unroll
-                for (int k = 0; k < 16; ++k) v[k] = hist[(int64_t)min(b0 + 4 * k, tiles - 1) * 256 + d];
+                for (int k = 0; k < 16; ++k) v[k] = hist[(int64_t)min(b0 + 8 * k, tiles - 1) * 128 + d];
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
-                    const int b = b0 + 4 * k;
-                    t += b < tiles ? v[k] : 0;
-                    p += b < (int)blockIdx.x ? v[k] : 0;
+                    const int b = b0 + 8 * k;
+                    const uint32_t w2 = b < tiles ? v[k] : 0, e2 = b < (int)blockIdx.x ? v[k] : 0;
+                    a0 += w2 & 0xffff;
+                    a1 += w2 >> 16;
+                    p0 += e2 & 0xffff;
+                    p1 += e2 >> 16;
                 }
             }
         }
-        pre[q][d] = p;
-        all[q][d] = t;
+        pre[q][d] = p0;
+        pre[q][d + 128] = p1;
+        all[q][d] = a0;
+        all[q][d + 128] = a1;
     }
 #pragma unroll
     for (int k = 0; k < KPT; ++k) dig[k] = (kk[k] >> shift) & 255;
     radix_rank<KPT>(dig, val, rank, L);  // (its barriers cover pre and all)
-    digit_scan(L.tot, L);                // base: the digit's first place in the tile
+    if (threadIdx.x < 512) {
+        uint32_t(*src)[256] = threadIdx.x < 256 ? pre : all;
+        const int d = threadIdx.x & 255;
+        uint32_t t = 0;
 #pragma unroll
-    for (int k = 0; k < KPT; ++k)
-        if (val[k]) sh[L.base[dig[k]] + L.wh[w][dig[k]] + rank[k]] = make_uint2(kk[k], ii[k]);
-    if (threadIdx.x < 256) {
-        const int d = threadIdx.x;
-        pre[0][d] = pre[0][d] + pre[1][d] + pre[2][d] + pre[3][d] - L.base[d];
-        all[0][d] = all[0][d] + all[1][d] + all[2][d] + all[3][d];
+        for (int q = 0; q < 8; ++q) t += src[q][d];
+        if (threadIdx.x < 256) pre[0][d] = t;
+        else L.tot[1][d] = t;
     }
     __syncthreads();
-    digit_scan(all[0], L);  // base: the digit's first place of all
+    digit_scan(L);  // base: the digit's first place in the tile, and of all
+#pragma unroll
+    for (int k = 0; k < KPT; ++k)
+        if (val[k]) sh[L.base[0][dig[k]] + L.wh[w][dig[k]] + rank[k]] = make_uint2(kk[k], ii[k]);
+    __syncthreads();
     const int n = T - t0 < RTILE ? (int)(T - t0) : RTILE;
     for (int j = threadIdx.x; j < n; j += RTHR) {
         const uint2 v = sh[j];
         const uint32_t d = (v.x >> shift) & 255;
-        kv2[L.base[d] + pre[0][d] + (uint32_t)j] = v;  // (modulo 2^32: pre may be "negative")
+        kv2[L.base[1][d] + pre[0][d] + ((uint32_t)j - L.base[0][d])] = v;
     }
 }
 
@@ -709,7 +723,7 @@ struct EmbPlan {
     bool few;
     int tpr, gb, tg, slices;
     int64_t pieces, tiles, Np;
-    int64_t o_kv[2], o_hist, o_part, bytes;
+    int64_t o_kv[2], o_hist, o_before, o_part, bytes;
 };
 static EmbPlan emb_plan(int64_t T, int64_t N, int64_t V) {
     EmbPlan q;
@@ -736,7 +750,8 @@ static EmbPlan emb_plan(int64_t T, int64_t N, int64_t V) {
     };
     if (!q.few)
         for (int i = 0; i < (T <= RONE ? 1 : 2); ++i) q.o_kv[i] = take(T * 8);
-    q.o_hist = take(q.few ? q.pieces * V * 4 : (q.tiles + 1) * 256 * 4);
+    q.o_hist = take(q.few ? q.pieces * V * 4 : q.tiles * 128 * 4);
+    q.o_before = take(!q.few && q.tiles > RFUSE ? (q.tiles + 1) * 256 * 4 : 0);
     q.o_part = take(q.pieces * (q.few ? V : 2) * q.Np * 4);
     q.bytes = o;
     return q;
@@ -763,15 +778,16 @@ hipError_t emb_bwd(const mmvae_embedding_args& a, hipStream_t st) {
     if (!q.few && a.T <= RONE) {
         OPCHK(launch(k_emb_sort1, dim3((unsigned)(1 + clear)), dim3(RTHR), st, a.ids, a.ids64, (int)a.T, V, passes, kv[0], a.dtable, out_bytes));
     } else if (!q.few) {
-        const int tiles = (int)q.tiles, scanned = tiles > RFUSE ? 1 : 0;
+        const int tiles = (int)q.tiles;
+        uint32_t* before = tiles > RFUSE ? (uint32_t*)(ws + q.o_before) : nullptr;
         for (int p = 0; p < passes; ++p) {
             const uint2* from = p ? kv[cur] : nullptr;
             const int nxt = p ? cur ^ 1 : 0;
             OPCHK(launch(k_emb_hist, dim3((unsigned)(tiles + (p ? 0 : clear))), dim3(RTHR), st, a.ids, a.ids64, from, a.T, V, 8 * p, tiles,
                          hist, a.dtable, out_bytes));
-            if (scanned) OPCHK(launch(k_emb_scan, dim3(256), dim3(256), st, tiles, hist));
-            OPCHK(launch(k_emb_scatter, dim3((unsigned)tiles), dim3(RTHR), st, a.ids, a.ids64, from, a.T, V, 8 * p, tiles, scanned,
-                         (const uint32_t*)hist, kv[nxt]));
+            if (before) OPCHK(launch(k_emb_scan, dim3(256), dim3(256), st, tiles, (const uint32_t*)hist, before));
+            OPCHK(launch(k_emb_scatter, dim3((unsigned)tiles), dim3(RTHR), st, a.ids, a.ids64, from, a.T, V, 8 * p, tiles,
+                         (const uint32_t*)hist, (const uint32_t*)before, kv[nxt]));
             cur = nxt;
         }
     }
