@@ -17,13 +17,14 @@ struct NormP {
     int64_t ldx, lddy, ldy;  // ldy: of y, or of dx
     void* y;                 // y, or dx
     float *mean, *rstd;
-    float* part;             // backward: the workgroups' sums [grid][2][Np]; null: one workgroup writes
-    void *dw, *db;           //   dw / db (or there are none)
+    float* part;             // backward: the workgroups' sums [grid][2][Np], or null
+    void *dw, *db;           // written by the strips
     int64_t Np;
     float eps;
     int relu;
     bool wf32;
     bool b_lds;              // forward, weights in LDS: the biases too
+    int strips;              // backward: the first workgroups, a strip of 8 columns each, sum dw and db
     DropKey drop;
 };
 
@@ -182,9 +183,74 @@ __global__ __launch_bounds__(BLK) void k_ln_fwd(NormP a) {
     }
 }
 
+// a strip of 8 columns summed over all rows by one workgroup: the row statistics are inputs, so this needs
+// nothing of what the row workgroups do.  Lane sums in each wave, then the waves in order.
+static constexpr int STRIP_BLK = 512;
+template <class T, bool MASK, bool EVEN> MMVAE_DEV void ln_strip(const NormP& a, float ds) {
+    __shared__ float sh[STRIP_BLK / 64][17];
+    // (workgroups go round the 8 XCDs: neighbouring strips, which share cache lines, to the same one)
+    const int c = (int)(blockIdx.x & 7) * (a.strips >> 3) + (int)(blockIdx.x >> 3), col = c * 8, N = a.N, n = N - col;
+    if (n <= 0) return;
+    float w[8], b[8], aw[8] = {}, ab[8] = {};
+    if (MASK) {
+        ldws<T>(a.w, a.wf32, col, n, 1.f, ds, w);
+        ldws<T>(a.b, a.wf32, col, n, 0.f, ds, b);
+    }
+    for (int64_t r0 = threadIdx.x; r0 < a.M; r0 += 2 * STRIP_BLK) {  // two rows at once
+        Chunk<T> x[2], d[2];
+        RowStat<T> st[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int64_t row = r0 + STRIP_BLK * k, rr = row < a.M ? row : r0;
+            x[k] = ld_row<EVEN>((const T*)a.x + rr * a.ldx, col, N);
+            d[k] = ld_row<EVEN>((const T*)a.dy + rr * a.lddy, col, N);
+            st[k].set(a.mean[rr], a.rstd[rr]);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int64_t row = r0 + STRIP_BLK * k;
+            if (row >= a.M) break;
+            if (MASK) {
+                bool on[8] = {true, true, true, true, true, true, true, true};
+                if (a.drop.thr) keep8(a.drop, row, c, on);
+                if (a.relu) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) on[i] = on[i] && st[k].u(x[k].get(i), w[i], b[i]) > 0.f;
+                }
+                d[k].keep(on);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float v = d[k].get(i);
+                aw[i] = __builtin_fmaf(v, st[k].xh(x[k].get(i)), aw[i]);
+                ab[i] += v;
+            }
+        }
+    }
+    const int wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float s = lanes_sum<64>(aw[i]), t = lanes_sum<64>(ab[i]);
+        if ((threadIdx.x & 63) == 0) {
+            sh[wave][i] = s;
+            sh[wave][8 + i] = t;
+        }
+    }
+    __syncthreads();
+    const int i = threadIdx.x & 7;
+    void* o = threadIdx.x < 8 ? a.dw : a.db;
+    if (threadIdx.x >= 16 || i >= n || !o) return;
+    float v = 0.f;
+#pragma unroll
+    for (int q = 0; q < STRIP_BLK / 64; ++q) v += sh[q][threadIdx.x];
+    if (MASK) v *= ds;
+    if (a.wf32) ((float*)o)[col + i] = v;
+    else ((T*)o)[col + i] = (T)v;
+}
+
 // backward: du = dy m [u > 0], g = du w, dx = rstd (g - mean(g) - xh mean(g xh)); the workgroup's
-// sums of du xh and du over its rows (of the unscaled du: times the dropout factor once, at the end) (fixed order: a thread's rows, then the row groups) -> part, or
-// with one workgroup straight into dw / db.  Elements behind a row's end are loaded as 0 and add 0.
+// sums of du xh and du over its rows (of the unscaled du: times the dropout factor once, at the end; fixed
+// order: a thread's rows, then the row groups) -> part, if there is one.  Elements behind a row's end are loaded as 0 and add 0.
 template <class T, int TPR, int VPT, int BLK, bool MASK, bool EVEN>
 __global__ __launch_bounds__(BLK, BLK / 256) void k_ln_bwd(NormP a) {
     constexpr int RPB = BLK / TPR;
@@ -197,6 +263,12 @@ __global__ __launch_bounds__(BLK, BLK / 256) void k_ln_bwd(NormP a) {
     const int N = a.N, slots = (N + 7) / 8;
     const float inv = 1.f / (float)N, ds = MASK && a.drop.thr ? a.drop.s : 1.f;
     if (MASK) drop_state(a.drop);
+    int strips = 0;
+    if constexpr (BLK == STRIP_BLK) {
+        strips = a.strips;
+        if ((int)blockIdx.x < strips) return ln_strip<T, MASK, EVEN>(a, ds);
+    }
+    const int64_t first = (int64_t)((int)blockIdx.x - strips) * RPB;
     float hw[HOLD ? VPT : 1][8];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
@@ -211,7 +283,7 @@ __global__ __launch_bounds__(BLK, BLK / 256) void k_ln_bwd(NormP a) {
         for (int i = 0; i < 8; ++i) aw[j][i] = ab[j][i] = 0.f;
     // a row's x and dy, dy without what dropout and ReLU take away: du = ds dc, g = dc (ds w).  (AGAIN: each phase reads
     // them, the second with the first's bits)
-    const int64_t step = (int64_t)gridDim.x * RPB;
+    const int64_t step = (int64_t)((int)gridDim.x - strips) * RPB;
     Chunk<T> xc[AGAIN ? 1 : VPT], dc[AGAIN ? 1 : VPT], xn[PRE ? VPT : 1], dn[PRE ? VPT : 1];
     uint32_t bits[VPT];
     float mean = 0.f, rstd = 0.f, mean_n = 0.f, rstd_n = 0.f;
@@ -229,8 +301,8 @@ __global__ __launch_bounds__(BLK, BLK / 256) void k_ln_bwd(NormP a) {
             for (int j = 0; j < VPT; ++j) read(r, j, x[j], d[j]);
         }
     };
-    if constexpr (PRE) fetch((int64_t)blockIdx.x * RPB + grp, xn, dn, mean_n, rstd_n);
-    for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.M; r0 += step) {
+    if constexpr (PRE) fetch(first + grp, xn, dn, mean_n, rstd_n);
+    for (int64_t r0 = first; r0 < a.M; r0 += step) {
         const int64_t row = r0 + grp;
         const bool ok = row < a.M;
         if constexpr (PRE) {
@@ -339,19 +411,8 @@ __global__ __launch_bounds__(BLK, BLK / 256) void k_ln_bwd(NormP a) {
         }
         if constexpr (TPR > 64) __syncthreads();
     }
-    if (!a.part && !a.dw && !a.db) return;
-    // a column's sum: into the partials, or (one workgroup) rounded into the gradients
-    auto put = [&](int h, int c, float v) {
-        if (MASK) v *= ds;
-        if (a.part) {
-            a.part[((int64_t)blockIdx.x * 2 + h) * a.Np + c] = v;
-        } else if (c < N) {
-            void* o = h ? a.db : a.dw;
-            if (!o) return;
-            if (a.wf32) ((float*)o)[c] = v;
-            else ((T*)o)[c] = (T)v;
-        }
-    };
+    if (!a.part) return;
+    auto put = [&](int h, int c, float v) { a.part[((int64_t)((int)blockIdx.x - strips) * 2 + h) * a.Np + c] = MASK ? v * ds : v; };
     if constexpr (RPB == 1) {
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
@@ -561,28 +622,29 @@ template <class F> inline hipError_t by_width(int N, F&& f) {
     if (nc <= 128) return f(I<64>{}, I<2>{}, I<256>{});
     if (nc <= 256) return f(I<256>{}, I<1>{}, I<256>{});
     if (nc <= 512) return f(I<256>{}, I<2>{}, I<256>{});
-    if (nc <= 1024) return f(I<512>{}, I<2>{}, I<512>{});
-    if (nc <= 1536) return f(I<512>{}, I<3>{}, I<512>{});
-    if (nc <= 2048) return f(I<512>{}, I<4>{}, I<512>{});
-    if (nc <= 2560) return f(I<512>{}, I<5>{}, I<512>{});
-    if (nc <= 3072) return f(I<512>{}, I<6>{}, I<512>{});
+    if (nc <= 512 * 2) return f(I<512>{}, I<2>{}, I<512>{});
+    if (nc <= 512 * 3) return f(I<512>{}, I<3>{}, I<512>{});
+    if (nc <= 512 * 4) return f(I<512>{}, I<4>{}, I<512>{});
+    if (nc <= 512 * 5) return f(I<512>{}, I<5>{}, I<512>{});
+    if (nc <= 512 * 6) return f(I<512>{}, I<6>{}, I<512>{});
     return f(I<512>{}, I<8>{}, I<512>{});
 }
-// a backward of few rows in one workgroup of 1024, which writes dw and db itself: rows it may have
-constexpr int ONE_ROUNDS = 2, LONG_PARTS = 128;
-inline bool norm_one(int64_t M, int64_t N) {
-    const int nc = (int)((std::min<int64_t>(N, LONG_N) + 7) / 8);
-    int tpr = 8;
-    while (tpr < 64 && tpr < nc) tpr *= 2;
-    return N <= 1024 ? M <= ONE_ROUNDS * (1024 / tpr) : N <= LONG_N && M <= 1;
-}
-template <class F> inline hipError_t by_width_one(int N, F&& f) {
+// (backward with masks: above 20,480 columns the sums do not stay in the registers, 228 bytes a lane spilled)
+constexpr int LONG_PARTS = 128, STRIP_ROWS = 2048, FITS_N = 20480;
+// A short backward sums dw and db in strips of columns, which read x and dy a second time, beside the
+// row workgroups of the same launch: no partial sums and no second launch to add them up.  us of both
+// (bf16, calls back to back): 100 x 128 2.6 / 5.2, 1024 x 1024 4.3 / 7.6, 1024 x 4096 11.2 / 25.1, 100 x
+// 20000 20.6 / 34.6; past the limits the second reading costs more: 4096 x 128 6.4 / 5.9, 2048 x 8192
+// 33.6 / 31.7, 4096 x 1024 13.0 / 11.5.
+inline bool norm_strips(int64_t M, int64_t N) { return M <= STRIP_ROWS && N <= FITS_N && M * N <= (1 << 22); }
+template <class F> inline hipError_t by_width_strips(int N, F&& f) {
     const int nc = (N + 7) / 8;
-    if (nc <= 8) return f(I<8>{}, I<1>{}, I<1024>{});
-    if (nc <= 16) return f(I<16>{}, I<1>{}, I<1024>{});
-    if (nc <= 32) return f(I<32>{}, I<1>{}, I<1024>{});
-    if (nc <= 64) return f(I<64>{}, I<1>{}, I<1024>{});
-    if (nc <= 128) return f(I<64>{}, I<2>{}, I<1024>{});
+    if (nc <= 8) return f(I<8>{}, I<1>{}, I<STRIP_BLK>{});
+    if (nc <= 16) return f(I<16>{}, I<1>{}, I<STRIP_BLK>{});
+    if (nc <= 32) return f(I<32>{}, I<1>{}, I<STRIP_BLK>{});
+    if (nc <= 64) return f(I<64>{}, I<1>{}, I<STRIP_BLK>{});
+    if (nc <= 128) return f(I<64>{}, I<2>{}, I<STRIP_BLK>{});
+    if (nc <= 512) return f(I<512>{}, I<1>{}, I<STRIP_BLK>{});
     return by_width(N, f);
 }
 inline NormP norm_p(const mmvae_norm_args& a) {
@@ -613,13 +675,12 @@ inline int norm_rpb(int64_t N) {  // rows a workgroup holds at once
 }
 // workgroups of the backward = rows of partial weight sums
 inline int64_t norm_parts(int64_t M, int64_t N) {
-    if (norm_one(M, N)) return 1;
     if (N > LONG_N) return std::min<int64_t>(M, LONG_PARTS);
     const int64_t need = (M + norm_rpb(N) - 1) / norm_rpb(N);
     return std::min<int64_t>(need, N > 4096 ? 256 : 512);
 }
 inline int64_t norm_ws_bytes(int64_t M, int64_t N) {
-    if (norm_one(M, N)) return 0;
+    if (norm_strips(M, N)) return 0;
     return norm_parts(std::max<int64_t>(M, 1), N) * 2 * ((N + 7) / 8 * 8) * (int64_t)sizeof(float);
 }
 
@@ -655,29 +716,50 @@ template <class T> hipError_t norm_bwd_t(const mmvae_norm_args& a, hipStream_t s
     p.lddy = a.lddy;
     p.y = a.dx;
     p.ldy = a.lddx;
-    const bool wg = a.dw || a.db, one = norm_one(a.M, a.N) && a.M > 0;
-    p.part = wg && !one ? (float*)a.ws : nullptr;
+    const bool wg = a.dw || a.db, strips = wg && norm_strips(a.M, a.N);
+    p.part = wg && !strips ? (float*)a.ws : nullptr;
     p.dw = a.dw;
     p.db = a.db;
-    // (with masks the sums of more than 20,480 columns do not stay in the registers: 228 bytes a lane spilled)
-    const bool sweeps = a.N > LONG_N || (!one && a.N > 20480 && (p.relu || p.drop.thr));
+    const bool sweeps = a.N > LONG_N || (a.N > FITS_N && (p.relu || p.drop.thr));
     const int64_t G = sweeps ? std::min<int64_t>(a.M, LONG_PARTS) : norm_parts(a.M, a.N);
+    // dx over dy or x: not beside strips that read them
+    auto clear = [&](const void* q, int64_t ld) {
+        const int64_t es = a.dtype == MMVAE_T_F32 ? 4 : 2;
+        const uintptr_t o = (uintptr_t)a.dx, i = (uintptr_t)q;
+        return o + ((a.M - 1) * a.lddx + a.N) * es <= i || i + ((a.M - 1) * ld + a.N) * es <= o;
+    };
+    const bool apart = !a.dx || a.M < 1 || (clear(a.x, a.ldx) && clear(a.dy, a.lddy));
+    auto go = [&](auto t, auto v, auto b) -> hipError_t {
+        return by_flags(p, [&](auto m, auto e) {
+            if constexpr (m.value && t.value * v.value * 8 > FITS_N) return hipErrorInvalidValue;  // (sweeps)
+            else {
+                const size_t lds = LnKeep<T, v.value, b.value, m.value, e.value>::B_HOLD ? 0 : (size_t)p.Np * 4;
+                constexpr int RPB = b.value / t.value;
+                const int64_t rows = strips ? (a.dx ? (a.M + RPB - 1) / RPB : 0) : G;
+                const auto k = k_ln_bwd<T, t.value, v.value, b.value, m.value, e.value>;
+                if (p.strips && apart) return launch_lds(lds, k, dim3((unsigned)(p.strips + rows)), dim3(b.value), st, p);
+                if (p.strips) {
+                    OPCHK(launch_lds(lds, k, dim3((unsigned)p.strips), dim3(b.value), st, p));
+                    p.strips = 0;
+                }
+                return rows ? launch_lds(lds, k, dim3((unsigned)rows), dim3(b.value), st, p) : hipSuccess;
+            }
+        });
+    };
+    if (a.M > 0 && strips) {
+        p.strips = (int)((p.Np / 8 + 7) / 8 * 8);
+        return by_width_strips(p.N, go);
+    }
     if (a.M > 0 && (a.dx || wg)) {
         if (sweeps) {
             if (wg)  // (first: dx may overwrite dy or x)
                 OPCHK(launch(k_ln_cols<T>, dim3((unsigned)((p.Np / 8 + 255) / 256), (unsigned)G), dim3(256), st, p));
             if (a.dx) OPCHK(launch(k_ln_bwd_long<T>, dim3((unsigned)std::min<int64_t>(a.M, 512)), dim3(1024), st, p));
         } else {
-            auto go = [&](auto t, auto v, auto b) -> hipError_t {
-                return by_flags(p, [&](auto m, auto e) {
-                    const size_t lds = LnKeep<T, v.value, b.value, m.value, e.value>::B_HOLD ? 0 : (size_t)p.Np * 4;
-                    return launch_lds(lds, k_ln_bwd<T, t.value, v.value, b.value, m.value, e.value>, dim3((unsigned)G), dim3(b.value), st, p);
-                });
-            };
-            OPCHK(one ? by_width_one(p.N, go) : by_width(p.N, go));
+            OPCHK(by_width(p.N, go));
         }
     }
-    if (!wg || one) return hipSuccess;
+    if (!wg) return hipSuccess;
     const dim3 grid((unsigned)((2 * p.Np + 31) / 32));
     const int parts = (int)(a.M > 0 ? G : 0);
     if (p.wf32)

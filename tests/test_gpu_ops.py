@@ -218,6 +218,31 @@ def test_norm_in_place():
         assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N", [(2048, 9), (2049, 9), (513, 64), (1025, 129), (2048, 2048), (2048, 2049), (1023, 4097), (204, 20480), (205, 20480), (70, 20481)])
+def test_norm_gradients_in_strips_and_in_parts(M, N, dtype):
+    """Both sides of the limits up to which a backward sums its columns in strips beside the rows."""
+    x, dy, w, b = make(M, N, dtype)
+    check_norm(x, dy, w, b)
+    check_norm(x, dy, w, b, relu=True, p=0.3, seed=5, step=9)
+
+
+@pytest.mark.parametrize("M,N", [(1, 7), (100, 129), (700, 1024), (3, 9000), (300, 5000), (2500, 500)])
+@pytest.mark.parametrize("over", ["dy", "x"])
+def test_norm_backward_over_its_inputs(M, N, over):
+    x, dy, w, b = make(M, N, BF16)
+    x, dy = x.contiguous(), dy.contiguous()
+    _, mean, rstd = ops.layer_norm_forward(x, w, b)
+    dx, dw, db = ops.layer_norm_backward(dy, x, mean, rstd, w, b)
+    x2, dy2, dw2, db2 = x.clone(), dy.clone(), torch.empty_like(dw), torch.empty_like(db)
+    out = dy2 if over == "dy" else x2
+    n = mmvae_amd.lib().mmvae_layer_norm_bwd_ws(M, N)
+    ws = torch.empty(n, dtype=torch.uint8, device=DEV)
+    c_norm("mmvae_layer_norm_bwd", x2, w, b, mean=mean.data_ptr(), rstd=rstd.data_ptr(), dy=dy2.data_ptr(), lddy=N, dx=out.data_ptr(), lddx=N,
+           dw=dw2.data_ptr(), db=db2.data_ptr(), ws=ws.data_ptr() if n else 0, ws_bytes=n)
+    assert torch.equal(out, dx) and torch.equal(dw2, dw) and torch.equal(db2, db)
+
+
 def test_norm_leaves_what_is_beside_its_rows():
     """Outputs with a row stride above N: the columns between the rows stay as they were."""
     M, N, ld = 37, 101, 120
