@@ -629,6 +629,12 @@ template <class F> inline hipError_t by_width(int N, F&& f) {
     if (nc <= 512 * 6) return f(I<512>{}, I<6>{}, I<512>{});
     return f(I<512>{}, I<8>{}, I<512>{});
 }
+// The backward's own: rows of 3521 .. 4096 on 512 threads, so that as many waves leave half the partial
+// sums (4096 x 4096 bf16 31.4 -> 26.0 us; at 3300 columns the idle lanes cost more, 8192 rows 49 -> 56 us)
+constexpr int HALF_N = 3520;
+template <class F> inline hipError_t by_width_bwd(int N, F&& f) {
+    return N > HALF_N && N <= 4096 ? f(I<512>{}, I<1>{}, I<512>{}) : by_width(N, f);
+}
 // (backward with masks: above 20,480 columns the sums do not stay in the registers, 228 bytes a lane spilled)
 constexpr int LONG_PARTS = 128, STRIP_ROWS = 2048, FITS_N = 20480;
 // A short backward sums dw and db in strips of columns, which read x and dy a second time, beside the
@@ -677,7 +683,7 @@ inline int norm_rpb(int64_t N) {  // rows a workgroup holds at once
 inline int64_t norm_parts(int64_t M, int64_t N) {
     if (N > LONG_N) return std::min<int64_t>(M, LONG_PARTS);
     const int64_t need = (M + norm_rpb(N) - 1) / norm_rpb(N);
-    return std::min<int64_t>(need, N > 4096 ? 256 : 512);
+    return std::min<int64_t>(need, N > HALF_N ? 256 : 512);
 }
 inline int64_t norm_ws_bytes(int64_t M, int64_t N) {
     if (norm_strips(M, N)) return 0;
@@ -756,7 +762,7 @@ template <class T> hipError_t norm_bwd_t(const mmvae_norm_args& a, hipStream_t s
                 OPCHK(launch(k_ln_cols<T>, dim3((unsigned)((p.Np / 8 + 255) / 256), (unsigned)G), dim3(256), st, p));
             if (a.dx) OPCHK(launch(k_ln_bwd_long<T>, dim3((unsigned)std::min<int64_t>(a.M, 512)), dim3(1024), st, p));
         } else {
-            OPCHK(by_width(p.N, go));
+            OPCHK(by_width_bwd(p.N, go));
         }
     }
     if (!wg) return hipSuccess;

@@ -219,7 +219,7 @@ def test_norm_in_place():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("M,N", [(2048, 9), (2049, 9), (513, 64), (1025, 129), (2048, 2048), (2048, 2049), (1023, 4097), (204, 20480), (205, 20480), (70, 20481)])
+@pytest.mark.parametrize("M,N", [(2048, 9), (2049, 9), (513, 64), (1025, 129), (2048, 2048), (2048, 2049), (1023, 4097), (204, 20480), (205, 20480), (70, 20481), (1200, 3520), (1200, 3521), (1100, 4096)])
 def test_norm_gradients_in_strips_and_in_parts(M, N, dtype):
     """Both sides of the limits up to which a backward sums its columns in strips beside the rows."""
     x, dy, w, b = make(M, N, dtype)
