@@ -36,7 +36,9 @@ MMVAE_DEV int64_t walk_row(const Walk& w, int u, int* chunk) {
 static int64_t walk_blocks(int64_t rows, int64_t N) { return (rows * ((N + 7) / 8) + 256 * WALK - 1) / (256 * WALK); }
 
 // =======================================================================================
-// Dropout alone
+// Dropout alone.  Bound by memory: 4096 x 20000 bf16 (328 MB) 58 us, 5.6 TB/s (part of the input comes from
+// the last-level cache); the mask's 20 products for 8 elements stay below the loads' time, its four chunks a
+// thread in flight are what the rate needs (one row a workgroup, as it was first, 66 us).
 // =======================================================================================
 template <class T>
 __global__ __launch_bounds__(256) void k_dropout(int64_t M, int N, const T* x, int64_t ldx, T* y, int64_t ldy, DropKey k) {
@@ -62,7 +64,9 @@ __global__ __launch_bounds__(256) void k_dropout(int64_t M, int N, const T* x, i
 }
 
 // =======================================================================================
-// Embedding: y[t] = scale table[id_t] (+ add[t]), zero rows for ids outside [0, V)
+// Embedding: y[t] = scale table[id_t] (+ add[t]), zero rows for ids outside [0, V).  Bound by the rows
+// written and the table rows read, of which hot ones come from L2: 262144 x 128 bf16 16 us (67 MB written,
+// 4.2 TB/s), 50001 x 517 f16 19 us (52 MB).
 // =======================================================================================
 struct EmbF {
     int64_t T;
@@ -121,14 +125,23 @@ template <class T> __global__ __launch_bounds__(256) void k_emb_fwd(EmbF a) {
 // Few rows (labels: V <= FEW), where a sort of all tokens would cost more than their sums: each
 // piece sorts its own tokens and leaves one partial per row it has (k_emb_seg<FEW>), and
 // k_emb_few_join adds them up in order.
+// No atomics on sums: equal calls give equal bits.  dy is read once; what is left beside it is the sort,
+// a chain of short kernels.  262144 tokens into 20000 x 128 bf16: histograms 4.4 + 3.9 us, scatters 2 x 7.5,
+// k_emb_seg 15.8 (67 MB of dy, 4.2 TB/s), k_emb_join 4.3.  50001 into 30011 x 517 f16: 6.6 (with the 31 MB
+// of zeros) + 3.6, 2 x 6.7, 23.4 (52 MB in rows that end inside a cache line), 4.8.  4096 labels into 12 x
+// 128 f32: 5.8 + 3.4.
 // =======================================================================================
-static constexpr int FEW = 64;
+static constexpr int FEW = 64;      // (128 columns bf16, 64 rows against 65 sorted: 256 tokens 8.2 / 12.2 us, 4096
+                                    // 8.9 / 15.3, 32768 16.2 / 18.3, 262144 30.5 / 28.9)
 static constexpr int RTHR = 1024;   // a sort tile: 16 waves x KPT x 64 tokens
-static constexpr int RONE = 4096;   // tokens that one workgroup sorts (KPT = 4)
-static constexpr int RTILE = 2048;  // a tile of a longer sort (KPT = 2)
-static constexpr int RFUSE = 256;   // up to so many tiles a scatter workgroup sums the histograms itself
+static constexpr int RONE = 4096;   // tokens that one workgroup sorts, KPT = 4 (4096 tokens into 20000 x 128 bf16
+                                    // 19.4 us, 4097 in tiles 24.9)
+static constexpr int RTILE = 2048;  // a tile of a longer sort, KPT = 2 (a scatter of 262144 tokens 7.5 us, with tiles of
+                                    // 1024 or 4096 9.2; of 50001 tokens 6.7, 1024 5.9, 4096 8.6)
+static constexpr int RFUSE = 256;   // up to so many tiles a scatter workgroup sums the histograms itself: a
+                                    // launch less (64 columns: 524288 tokens 47.4 us, one more 51.7)
 
-// stable ranks of the workgroup's keys by an 8-bit digit (16 waves, KPT keys a lane; wave w holds the
+// Stable ranks of the workgroup's keys by an 8-bit digit (16 waves, KPT keys a lane; wave w holds the
 // tokens w 64 KPT + k 64 + lane).  wh[w][d]: first the wave's counts, then the count of d in earlier waves.
 struct RadixLds {
     uint32_t wh[RTHR / 64][256];
@@ -211,7 +224,8 @@ MMVAE_DEV void fill_zero(void* out, int64_t bytes, int64_t i, int64_t step) {
     for (; i < n; i += step) q[i] = make_uint4(0, 0, 0, 0);
 }
 
-// the whole sort of T <= RONE tokens in workgroup 0; the others clear the gradient
+// the whole sort of T <= RONE tokens in workgroup 0, the keys in registers from pass to pass (a chain of LDS
+// round trips: 10 us for two digits of 4096 tokens, 6 for one); the others clear the gradient
 __global__ __launch_bounds__(RTHR) void k_emb_sort1(const void* ids, int i64, int T, uint32_t V, int passes, uint2* kv, void* out,
                                                     int64_t out_bytes) {
     if (blockIdx.x > 0) {
@@ -305,7 +319,8 @@ __global__ __launch_bounds__(256) void k_emb_scan(int tiles, const uint32_t* his
     if (threadIdx.x == 0) before[(int64_t)tiles * 256 + d] = carry;
 }
 // one pass: a tile's tokens, sorted by the digit in LDS first (so that a digit's tokens leave together),
-// to their places
+// to their places.  7.5 us for 128 tiles: one round of latencies (keys, histograms, ranks, scans), half of it
+// in the ranks' ballots and LDS counters
 __global__ __launch_bounds__(RTHR) void k_emb_scatter(const void* ids, int i64, const uint2* kv, int64_t T, uint32_t V, int shift, int tiles,
                                                       const uint32_t* hist, const uint32_t* before, uint2* kv2) {
     constexpr int KPT = RTILE / RTHR;
@@ -472,7 +487,8 @@ MMVAE_DEV int few_sort(const EmbB& a, int64_t p0, int P, uint32_t* sk, uint32_t*
     // (with V = FEW the ids outside count as FEW, with V < FEW as V: behind the rows either way)
     return (int)(a.V < FEW ? L.base[a.V] : L.base[FEW]);
 }
-// TPR lanes x 8 columns; the 256 / TPR groups of a workgroup take a.tg consecutive sorted tokens each
+// TPR lanes x 8 columns; the 256 / TPR groups of a workgroup take a.tg consecutive sorted tokens each, eight
+// rows of dy in flight.  The groups are cut by place, not by id, so a hot id costs no more than others.
 template <class T, int TPR, bool ISFEW> __global__ __launch_bounds__(256) void k_emb_seg(EmbB a) {
     constexpr int GB = 256 / TPR, U = 8;
     __shared__ float head[GB][TPR * 8], tail[GB][TPR * 8];
