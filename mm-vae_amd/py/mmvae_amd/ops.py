@@ -88,12 +88,14 @@ class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, p, seed, kw):
         ctx.key = (p, seed, kw)
+        ctx.save_for_backward(kw.get("state"))  # (changed before the backward: refused)
         return dropout_apply(x, p, seed, **kw)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         p, seed, kw = ctx.key
+        ctx.saved_tensors
         return dropout_apply(dy, p, seed, **kw), None, None, None
 
 

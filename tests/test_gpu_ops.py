@@ -266,6 +266,18 @@ def test_dropout_bits(M, N, pad, dtype):
         assert y.dtype == dtype and torch.equal(y, want), (p, seed)
 
 
+def test_state_changed_before_the_backward_is_refused():
+    x, _, w, b = make(9, 40, F32)
+    x.requires_grad_()
+    state = torch.zeros(2, dtype=torch.int64, device=DEV)
+    for f in (lambda: ops.dropout(x, 0.5, 3, state=state), lambda: ops.layer_norm(x, w, b, p=0.5, seed=3, state=state)):
+        y = f()
+        state += 1
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+        f().sum().backward()
+
+
 def test_dropout_same_mask_as_the_norm_and_backward():
     x, dy, w, b = make(200, 77, F32)
     key = dict(p=0.4, seed=1234, step=9, row_offset=3)
