@@ -35,7 +35,7 @@ struct NormP {
     int relu;
     bool wf32;
     bool b_lds;              // forward, weights in LDS: the biases too
-    int strips;              // backward: the first workgroups, a strip of 8 columns each, sum dw and db
+    int strips, strip_waves; // backward: the first workgroups sum dw and db in strips of 8 columns, so many waves each
     DropKey drop;
 };
 
@@ -195,32 +195,37 @@ __global__ __launch_bounds__(BLK) void k_ln_fwd(NormP a) {
     }
 }
 
-// a strip of 8 columns summed over all rows by one workgroup: the row statistics are inputs, so this needs
-// nothing of what the row workgroups do.  Lane sums in each wave, then the waves in order.
+// strips of 8 columns summed over all rows: the row statistics are inputs, so this needs nothing of what the
+// row workgroups do.  A workgroup's 8 waves sum one strip, or (rows above 4096 columns, where strips are many)
+// four strips: lane sums in each wave, then a strip's waves in order (256 x 20000 bf16, waves a strip: 8 24
+// us, 4 17.9, 2 16.8, 1 16.7; 512 rows with dropout: 4 39.9, 2 38.1, 1 39.8).
 static constexpr int STRIP_BLK = 512;
+static constexpr bool strips_beside(int chunks, bool mask) { return chunks <= (mask ? 512 : 1024); }
 template <class T, bool MASK, bool EVEN> MMVAE_DEV void ln_strip(const NormP& a, float ds) {
     __shared__ float sh[STRIP_BLK / 64][17];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, sw = a.strip_waves, each = STRIP_BLK / 64 / sw;
     // (workgroups go round the 8 XCDs: neighbouring strips, which share cache lines, to the same one)
-    const int c = (int)(blockIdx.x & 7) * (a.strips >> 3) + (int)(blockIdx.x >> 3), col = c * 8, N = a.N, n = N - col;
-    if (n <= 0) return;
+    const int c0 = ((int)(blockIdx.x & 7) * (a.strips >> 3) + (int)(blockIdx.x >> 3)) * each;
+    const int c = c0 + wave / sw, col = c * 8, N = a.N, n = N - col;
     float w[8], b[8], aw[8] = {}, ab[8] = {};
     if (MASK) {
         ldws<T>(a.w, a.wf32, col, n, 1.f, ds, w);
         ldws<T>(a.b, a.wf32, col, n, 0.f, ds, b);
     }
-    for (int64_t r0 = threadIdx.x; r0 < a.M; r0 += 2 * STRIP_BLK) {  // two rows at once
+    const int64_t step = 64 * sw;
+    for (int64_t r0 = (wave % sw) * 64 + lane; r0 < a.M && n > 0; r0 += 2 * step) {  // two rows at once
         Chunk<T> x[2], d[2];
         RowStat<T> st[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            const int64_t row = r0 + STRIP_BLK * k, rr = row < a.M ? row : r0;
+            const int64_t row = r0 + step * k, rr = row < a.M ? row : r0;
             x[k] = ld_row<EVEN>((const T*)a.x + rr * a.ldx, col, N);
             d[k] = ld_row<EVEN>((const T*)a.dy + rr * a.lddy, col, N);
             st[k].set(a.mean[rr], a.rstd[rr]);
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            const int64_t row = r0 + STRIP_BLK * k;
+            const int64_t row = r0 + step * k;
             if (row >= a.M) break;
             if (MASK) {
                 bool on[8] = {true, true, true, true, true, true, true, true};
@@ -239,25 +244,28 @@ template <class T, bool MASK, bool EVEN> MMVAE_DEV void ln_strip(const NormP& a,
             }
         }
     }
-    const int wave = threadIdx.x >> 6;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float s = lanes_sum<64>(aw[i]), t = lanes_sum<64>(ab[i]);
-        if ((threadIdx.x & 63) == 0) {
+        if (lane == 0) {
             sh[wave][i] = s;
             sh[wave][8 + i] = t;
         }
     }
     __syncthreads();
-    const int i = threadIdx.x & 7;
-    void* o = threadIdx.x < 8 ? a.dw : a.db;
-    if (threadIdx.x >= 16 || i >= n || !o) return;
+    const int k = threadIdx.x & 15, q0 = threadIdx.x >> 4, at = (c0 + q0) * 8 + (k & 7);
+    void* o = k < 8 ? a.dw : a.db;
+    if (q0 >= each || at >= N || !o) return;
     float v = 0.f;
-#pragma unroll
-    for (int q = 0; q < STRIP_BLK / 64; ++q) v += sh[q][threadIdx.x];
+    for (int q = q0 * sw; q < (q0 + 1) * sw; ++q) v += sh[q][k];
     if (MASK) v *= ds;
-    if (a.wf32) ((float*)o)[col + i] = v;
-    else ((T*)o)[col + i] = (T)v;
+    if (a.wf32) ((float*)o)[at] = v;
+    else ((T*)o)[at] = (T)v;
+}
+// the strips alone: of rows whose own kernel leaves room for one workgroup a CU, and where dx overwrites dy or x
+template <class T, bool MASK, bool EVEN> __global__ __launch_bounds__(STRIP_BLK) void k_ln_strips(NormP a) {
+    if (MASK) drop_state(a.drop);
+    ln_strip<T, MASK, EVEN>(a, MASK && a.drop.thr ? a.drop.s : 1.f);
 }
 
 // backward: du = dy m [u > 0], g = du w, dx = rstd (g - mean(g) - xh mean(g xh)); the workgroup's
@@ -279,7 +287,7 @@ __global__ __launch_bounds__(BLK, BLK / 256) void k_ln_bwd(NormP a) {
     const float inv = 1.f / (float)N, ds = MASK && a.drop.thr ? a.drop.s : 1.f;
     if (MASK) drop_state(a.drop);
     int strips = 0;
-    if constexpr (BLK == STRIP_BLK) {
+    if constexpr (BLK == STRIP_BLK && strips_beside(TPR * VPT, MASK)) {
         strips = a.strips;
         if ((int)blockIdx.x < strips) return ln_strip<T, MASK, EVEN>(a, ds);
     }
@@ -654,13 +662,14 @@ template <class F> inline hipError_t by_width_bwd(int N, F&& f) {
     return N > HALF_N && N <= 4096 ? f(I<512>{}, I<1>{}, I<512>{}) : by_width(N, f);
 }
 // (backward with masks: above 20,480 columns the sums do not stay in the registers, 228 bytes a lane spilled)
-constexpr int LONG_PARTS = 128, STRIP_ROWS = 2048, FITS_N = 20480;
-// A short backward sums dw and db in strips of columns, which read x and dy a second time, beside the
-// row workgroups of the same launch: no partial sums and no second launch to add them up.  us of both
-// (bf16, calls back to back): 100 x 128 2.6 / 5.2, 1024 x 1024 4.3 / 7.6, 1024 x 4096 11.2 / 25.1, 100 x
-// 20000 20.6 / 34.6; past the limits the second reading costs more: 4096 x 128 6.4 / 5.9, 2048 x 8192
-// 33.6 / 31.7, 4096 x 1024 13.0 / 11.5.
-inline bool norm_strips(int64_t M, int64_t N) { return M <= STRIP_ROWS && N <= FITS_N && M * N <= (1 << 22); }
+constexpr int LONG_PARTS = 128, FITS_N = 20480, STRIP_N = 4096;
+// A backward of few rows sums dw and db in strips of columns, which read x and dy a second time: no partial
+// sums to write, read and add up.  Up to 4096 columns (8192 without masks) they stand beside the row workgroups of
+// the same launch; longer rows' kernels leave room for one workgroup a CU, there the strips go first by
+// themselves.  us of both ways (bf16, calls back to back): 100 x 128 2.6 / 5.2, 1024 x 1024 4.7 / 7.6, 1024 x 4096
+// 11.2 / 25.1, 100 x 20000 10.8 / 34.6, 512 x 20000 31.8 / 48.0; past the limits the second reading costs more: 4096 x
+// 128 6.4 / 5.9, 4096 x 1024 13.0 / 11.5, 1024 x 10201 45.4 / 34.8.
+inline bool norm_strips(int64_t M, int64_t N) { return N <= STRIP_N ? M <= 2048 && M * N <= (1 << 22) : M <= 512; }
 template <class F> inline hipError_t by_width_strips(int N, F&& f) {
     const int nc = (N + 7) / 8;
     if (nc <= 8) return f(I<8>{}, I<1>{}, I<STRIP_BLK>{});
@@ -763,18 +772,23 @@ template <class T> hipError_t norm_bwd_t(const mmvae_norm_args& a, hipStream_t s
                 constexpr int RPB = b.value / t.value;
                 const int64_t rows = strips ? (a.dx ? (a.M + RPB - 1) / RPB : 0) : G;
                 const auto k = k_ln_bwd<T, t.value, v.value, b.value, m.value, e.value>;
-                if (p.strips && apart) return launch_lds(lds, k, dim3((unsigned)(p.strips + rows)), dim3(b.value), st, p);
+                if (p.strips && apart && strips_beside(t.value * v.value, m.value))
+                    return launch_lds(lds, k, dim3((unsigned)(p.strips + rows)), dim3(b.value), st, p);
                 if (p.strips) {
-                    OPCHK(launch_lds(lds, k, dim3((unsigned)p.strips), dim3(b.value), st, p));
+                    OPCHK(launch(k_ln_strips<T, m.value, e.value>, dim3((unsigned)p.strips), dim3(STRIP_BLK), st, p));
                     p.strips = 0;
                 }
                 return rows ? launch_lds(lds, k, dim3((unsigned)rows), dim3(b.value), st, p) : hipSuccess;
             }
         });
     };
-    if (a.M > 0 && strips) {
-        p.strips = (int)((p.Np / 8 + 7) / 8 * 8);
-        return by_width_strips(p.N, go);
+    if (a.M > 0 && strips) {  // (first: dx may overwrite dy or x)
+        p.strip_waves = a.N > STRIP_N ? 2 : STRIP_BLK / 64;
+        const int64_t each = STRIP_BLK / 64 / p.strip_waves;
+        p.strips = (int)((p.Np / 8 + 8 * each - 1) / (8 * each) * 8);
+        if (!sweeps) return by_width_strips(p.N, go);
+        OPCHK(by_flags(p, [&](auto m, auto e) { return launch(k_ln_strips<T, m.value, e.value>, dim3((unsigned)p.strips), dim3(STRIP_BLK), st, p); }));
+        return a.dx ? launch(k_ln_bwd_long<T>, dim3((unsigned)a.M), dim3(1024), st, p) : hipSuccess;
     }
     if (a.M > 0 && (a.dx || wg)) {
         if (sweeps) {

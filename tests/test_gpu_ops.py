@@ -219,7 +219,7 @@ def test_norm_in_place():
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("M,N", [(2048, 9), (2049, 9), (513, 64), (1025, 129), (2048, 2048), (2048, 2049), (1023, 4097), (204, 20480), (205, 20480), (70, 20481), (1200, 3520), (1200, 3521), (1100, 4096)])
+@pytest.mark.parametrize("M,N", [(2048, 9), (2049, 9), (513, 64), (1025, 129), (2048, 2048), (2048, 2049), (1023, 4097), (204, 20480), (512, 4097), (513, 4097), (129, 8193), (70, 20481), (3, 33001), (1200, 3520), (1200, 3521), (1100, 4096)])
 def test_norm_gradients_in_strips_and_in_parts(M, N, dtype):
     """Both sides of the limits up to which a backward sums its columns in strips beside the rows."""
     x, dy, w, b = make(M, N, dtype)
@@ -227,7 +227,7 @@ def test_norm_gradients_in_strips_and_in_parts(M, N, dtype):
     check_norm(x, dy, w, b, relu=True, p=0.3, seed=5, step=9)
 
 
-@pytest.mark.parametrize("M,N", [(1, 7), (100, 129), (700, 1024), (3, 9000), (300, 5000), (2500, 500)])
+@pytest.mark.parametrize("M,N", [(1, 7), (100, 129), (700, 1024), (3, 9000), (300, 5000), (2500, 500), (600, 5000), (40, 21001)])
 @pytest.mark.parametrize("over", ["dy", "x"])
 def test_norm_backward_over_its_inputs(M, N, over):
     x, dy, w, b = make(M, N, BF16)

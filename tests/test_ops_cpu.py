@@ -115,7 +115,7 @@ def test_workspace_sizes_grow_with_the_call():
     for N in (1, 7, 64, 100, 1000, 20000, 32768, 32769, 100000):
         for M in (0, 1, 2, 100, 2048, 4096):  # few rows: columns summed in strips, no partial sums
             n = L.mmvae_layer_norm_bwd_ws(M, N)
-            assert n >= 2 * 4 * N or (n == 0 and M <= 2048 and M * N <= 1 << 22)
+            assert n >= 2 * 4 * N or (n == 0 and (M <= 512 or M <= 2048 and M * N <= 1 << 22))
         assert L.mmvae_layer_norm_bwd_ws(4096, N) > 0
     # the sorted tokens (id, place), and a partial head and tail of a piece at least
     for T in (1, 4096, 4097, 600000):
