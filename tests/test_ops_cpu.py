@@ -77,7 +77,7 @@ def test_norm_forward_refuses(kw):
 
 
 @pytest.mark.parametrize("kw", NORM_BAD + [dict(dy=0), dict(mean=0), dict(rstd=0), dict(lddx=7), dict(M=5000, ws=0),
-                                            dict(M=5000, ws_bytes=8), dict(lddy=-8)])
+                                            dict(M=5000, ws_bytes=8), dict(lddy=-8), dict(M=1, N=2 ** 26)])
 def test_norm_backward_refuses(kw):
     assert mmvae_amd.lib().mmvae_layer_norm_bwd(pack_norm(**kw)) == -1
 
