@@ -200,7 +200,6 @@ __global__ __launch_bounds__(BLK) void k_ln_fwd(NormP a) {
 // four strips: lane sums in each wave, then a strip's waves in order (256 x 20000 bf16, waves a strip: 8 24
 // us, 4 17.9, 2 16.8, 1 16.7; 512 rows with dropout: 4 39.9, 2 38.1, 1 39.8).
 static constexpr int STRIP_BLK = 512;
-static constexpr bool strips_beside(int chunks, bool mask) { return chunks <= (mask ? 512 : 1024); }
 template <class T, bool MASK, bool EVEN> MMVAE_DEV void ln_strip(const NormP& a, float ds) {
     __shared__ float sh[STRIP_BLK / 64][17];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, sw = a.strip_waves, each = STRIP_BLK / 64 / sw;
@@ -262,7 +261,7 @@ template <class T, bool MASK, bool EVEN> MMVAE_DEV void ln_strip(const NormP& a,
     if (a.wf32) ((float*)o)[at] = v;
     else ((T*)o)[at] = (T)v;
 }
-// the strips alone: of rows whose own kernel leaves room for one workgroup a CU, and where dx overwrites dy or x
+// the strips alone: of rows that are read in sweeps, and where dx overwrites dy or x
 template <class T, bool MASK, bool EVEN> __global__ __launch_bounds__(STRIP_BLK) void k_ln_strips(NormP a) {
     if (MASK) drop_state(a.drop);
     ln_strip<T, MASK, EVEN>(a, MASK && a.drop.thr ? a.drop.s : 1.f);
@@ -287,7 +286,7 @@ __global__ __launch_bounds__(BLK, BLK / 256) void k_ln_bwd(NormP a) {
     const float inv = 1.f / (float)N, ds = MASK && a.drop.thr ? a.drop.s : 1.f;
     if (MASK) drop_state(a.drop);
     int strips = 0;
-    if constexpr (BLK == STRIP_BLK && strips_beside(TPR * VPT, MASK)) {
+    if constexpr (BLK == STRIP_BLK) {
         strips = a.strips;
         if ((int)blockIdx.x < strips) return ln_strip<T, MASK, EVEN>(a, ds);
     }
@@ -663,12 +662,11 @@ template <class F> inline hipError_t by_width_bwd(int N, F&& f) {
 }
 // (backward with masks: above 20,480 columns the sums do not stay in the registers, 228 bytes a lane spilled)
 constexpr int LONG_PARTS = 128, FITS_N = 20480, STRIP_N = 4096;
-// A backward of few rows sums dw and db in strips of columns, which read x and dy a second time: no partial
-// sums to write, read and add up.  Up to 4096 columns (8192 without masks) they stand beside the row workgroups of
-// the same launch; longer rows' kernels leave room for one workgroup a CU, there the strips go first by
-// themselves.  us of both ways (bf16, calls back to back): 100 x 128 2.6 / 5.2, 1024 x 1024 4.7 / 7.6, 1024 x 4096
-// 11.2 / 25.1, 100 x 20000 10.8 / 34.6, 512 x 20000 31.8 / 48.0; past the limits the second reading costs more: 4096 x
-// 128 6.4 / 5.9, 4096 x 1024 13.0 / 11.5, 1024 x 10201 45.4 / 34.8.
+// A backward of few rows sums dw and db in strips of columns, beside the row workgroups of the same launch: x
+// and dy are read a second time, but there are no partial sums to write, read and add up.  us of both ways
+// (bf16, calls back to back): 100 x 128 2.6 / 5.2, 1024 x 1024 4.7 / 7.6, 1024 x 4096 11.2 / 25.1, 100 x 20000
+// 10.2 / 34.6, 512 x 20000 27.5 / 48.0; past the limits the second reading costs more: 4096 x 128 6.4 / 5.9,
+// 4096 x 1024 13.0 / 11.5, 1024 x 16800 with dropout 57 / 57.
 inline bool norm_strips(int64_t M, int64_t N) { return N <= STRIP_N ? M <= 2048 && M * N <= (1 << 22) : M <= 512; }
 template <class F> inline hipError_t by_width_strips(int N, F&& f) {
     const int nc = (N + 7) / 8;
@@ -772,7 +770,7 @@ template <class T> hipError_t norm_bwd_t(const mmvae_norm_args& a, hipStream_t s
                 constexpr int RPB = b.value / t.value;
                 const int64_t rows = strips ? (a.dx ? (a.M + RPB - 1) / RPB : 0) : G;
                 const auto k = k_ln_bwd<T, t.value, v.value, b.value, m.value, e.value>;
-                if (p.strips && apart && strips_beside(t.value * v.value, m.value))
+                if (p.strips && apart)
                     return launch_lds(lds, k, dim3((unsigned)(p.strips + rows)), dim3(b.value), st, p);
                 if (p.strips) {
                     OPCHK(launch(k_ln_strips<T, m.value, e.value>, dim3((unsigned)p.strips), dim3(STRIP_BLK), st, p));
