@@ -22,7 +22,6 @@ import numpy as np
 import torch
 
 own = False
-_module = None
 
 _TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 _SIZE = {"f32": 4, "bf16": 2, "f16": 2}
@@ -30,16 +29,11 @@ _EPS = 1e-5
 
 
 def _ops():
-    """The framework's operators, imported once (as a program does, not in every pass)."""
-    global _module
-    if _module is not None:
-        return _module
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     path = os.path.join(root, "mm-vae_amd", "py")
     if path not in sys.path:
         sys.path.insert(0, path)
     from mmvae_amd import ops
-    _module = ops
     return ops
 
 
