@@ -320,6 +320,7 @@ typedef struct mmvae_norm_args {
 } mmvae_norm_args;
 int mmvae_layer_norm_fwd(const mmvae_norm_args* args);
 int mmvae_layer_norm_bwd(const mmvae_norm_args* args);
+/* enough for any fewer rows of N too */
 int64_t mmvae_layer_norm_bwd_ws(int64_t M, int64_t N);
 
 /* y[r][c] = x[r][c] times its dropout factor; a dropped element is 0 whatever x holds.  The
@@ -364,6 +365,7 @@ typedef struct mmvae_embedding_args {
 } mmvae_embedding_args;
 int mmvae_embedding_fwd(const mmvae_embedding_args* args);
 int mmvae_embedding_bwd(const mmvae_embedding_args* args);
+/* enough for any fewer tokens of the same table too */
 int64_t mmvae_embedding_bwd_ws(int64_t T, int64_t N, int64_t V);
 
 /* ---- operators.hh (vMF observation model scalars) ----------------------------------

@@ -735,6 +735,7 @@ hipError_t emb_fwd(const mmvae_embedding_args& a, hipStream_t st) {
 }
 
 // the gradient's plan, a function of (T, N, V) alone: tokens per group and pieces
+static constexpr int64_t SHORT_T = 32768;  // up to so many tokens a group takes 8
 struct EmbPlan {
     bool few;
     int tpr, gb, tg, slices;
@@ -754,8 +755,8 @@ static EmbPlan emb_plan(int64_t T, int64_t N, int64_t V) {
     q.gb = 256 / q.tpr;
     q.slices = (int)((nc + q.tpr - 1) / q.tpr);
     // a group's tokens: 8 in one go of loads; more for long inputs, so that the partials stay few beside dy
-    q.tg = T > 32768 ? 16 : 8;
-    if (q.few && T > 32768) q.tg = 512 / q.gb;
+    q.tg = T > SHORT_T ? 16 : 8;
+    if (q.few && T > SHORT_T) q.tg = 512 / q.gb;
     q.pieces = std::max<int64_t>(1, (T + (int64_t)q.gb * q.tg - 1) / ((int64_t)q.gb * q.tg));
     q.tiles = (T + RTILE - 1) / RTILE;
     int64_t o = 0;
@@ -772,7 +773,10 @@ static EmbPlan emb_plan(int64_t T, int64_t N, int64_t V) {
     q.bytes = o;
     return q;
 }
-int64_t emb_bwd_ws(int64_t T, int64_t N, int64_t V) { return T == 0 || V == 0 ? 0 : emb_plan(T, N, V).bytes; }
+static int64_t emb_need(int64_t T, int64_t N, int64_t V) { return T == 0 || V == 0 ? 0 : emb_plan(T, N, V).bytes; }
+// enough for T tokens and for any fewer: on each side of SHORT_T the need grows with T, but above it a group takes
+// more tokens, so that there are fewer partials (12 rows of 128: 32768 tokens 1.6 MB, 32769 0.4 MB)
+int64_t emb_bwd_ws(int64_t T, int64_t N, int64_t V) { return std::max(emb_need(T, N, V), emb_need(std::min(T, SHORT_T), N, V)); }
 
 __global__ __launch_bounds__(1024) void k_emb_clear(void* out, int64_t out_bytes) {
     fill_zero(out, out_bytes, (int64_t)blockIdx.x * 1024 + threadIdx.x, (int64_t)gridDim.x * 1024);
@@ -905,7 +909,7 @@ const char* emb_check(const mmvae_embedding_args& a, bool bwd) {
     if (a.V > 0 && !a.dtable) return "dtable is null";
     if (a.lddy < 0) return "dy's row stride is negative";
     if ((uintptr_t)a.dtable & 3) return "dtable must be 4-byte aligned";
-    if (emb_bwd_ws(a.T, a.N, a.V) > 0 && (!a.ws || a.ws_bytes < emb_bwd_ws(a.T, a.N, a.V)))
+    if (emb_need(a.T, a.N, a.V) > 0 && (!a.ws || a.ws_bytes < emb_need(a.T, a.N, a.V)))
         return "the workspace is below mmvae_embedding_bwd_ws(T, N, V) bytes";
     if (((uintptr_t)a.ws & 15) != 0) return "the workspace must be 16-byte aligned";
     return nullptr;

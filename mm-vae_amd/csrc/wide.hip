@@ -789,7 +789,8 @@ struct WideState {
     __bf16 *pl_F = nullptr, *pl_E = nullptr;
     int kp_F = 0, kp_E = 0;
     float* colv = nullptr;  // [D] the short-K GEMM's combined column constants
-    // layer operators (ops.hip): their workspace, and the decoder's input z + label_scale E[label]
+    // layer operators (ops.hip): their workspace, sized for the largest batch (the size functions cover every
+    // smaller one), and the decoder's input z + label_scale E[label]
     void* op_ws = nullptr;
     int64_t op_ws_bytes = 0;
     float* Zl = nullptr;
@@ -2556,7 +2557,7 @@ static hipError_t layer_bwd(Engine* e, const WLayer& L, int B, float* d) {
         a.db = e->greg(L.norm + ".bias");
         a.ws = e->wide_st->op_ws;
         a.ws_bytes = e->wide_st->op_ws_bytes;
-        return norm_bwd(a, e->stream);
+        return norm_check(a, true) ? hipErrorInvalidValue : norm_bwd(a, e->stream);
     }
     if (L.drop) {
         ScopedTimer tm(e, "w_dropout");
@@ -2823,6 +2824,7 @@ static hipError_t dec_backward(Engine* e, int B) {
         a.dtable = e->greg("label_embedding.weight");
         a.ws = w->op_ws;
         a.ws_bytes = w->op_ws_bytes;
+        if (emb_check(a, true)) return hipErrorInvalidValue;
         if ((er = emb_bwd(a, e->stream)) != hipSuccess) return er;
     }
     return hipGetLastError();

@@ -235,6 +235,23 @@ def test_label_refusals_and_states():
         e2.set_labels([0] * 50)
 
 
+@pytest.mark.parametrize("V", [5, 90])
+def test_small_batches_on_a_handle_for_large_ones(V):
+    """A batch of 20,000 and one of 32,768 on a handle for 40,000 (which has fewer, longer pieces of a label's tokens than
+    they have) give what a handle of their own size gives."""
+    kw = dict(D=70, V=V, enc_hidden=(12,), dec_hidden=(16,), layer_norm=True)
+    big = engine("nb", "f32", B=40000, **kw)
+    start = big.params(registered_only=True)
+    for B in (20000, 32768, 40000):
+        own = engine("nb", "f32", B=B, **kw)
+        cells = (np.arange(B, dtype=np.int64) * 7) % 400
+        eps = np.random.default_rng(B).standard_normal(B * (big.K + 1)).astype(np.float32)
+        big.set_params(start)
+        a, b = (e.step(cells, 0.7, eps=eps, step_id=3)[0] for e in (big, own))
+        assert abs(a - b) <= 2e-5 * abs(b), B
+        assert_grads_close(big.grads(), own.grads(), 2e-4, ctx=f"batch {B}")
+
+
 def test_dropout_draws_new_masks_each_step_and_none_in_encode():
     eng = engine("nb", "f32", V=0, dropout=0.5)
     cells, zero = np.arange(96), np.zeros(96 * (eng.K + 1), np.float32)

@@ -123,6 +123,24 @@ def test_workspace_sizes_grow_with_the_call():
         assert L.mmvae_embedding_bwd_ws(T, 33, 7) >= 7 * 4 * 40  # few rows: a partial of each
 
 
+@pytest.mark.parametrize("N", [1, 24, 64, 128, 136, 517, 1025])  # 8, 16 and 32 lanes a row
+@pytest.mark.parametrize("V", [1, 5, 12, 64, 65, 300, 30000])
+def test_embedding_workspace_covers_every_smaller_call(V, N):
+    """A workspace of the largest batch's size serves every smaller one (the engine keeps one): the size never falls
+    as the tokens grow, over the limits of one-workgroup sorts, of long inputs and of many tiles."""
+    L = mmvae_amd.lib()
+    T = sorted({max(1, c + d) for c in (0, 64, 512, 4096, 20000, 32768, 33024, 40000, 65536, 262144, 524288, 1 << 20) for d in (-1, 0, 1, 64)})
+    size = [L.mmvae_embedding_bwd_ws(t, N, V) for t in T]
+    assert all(a <= b for a, b in zip(size, size[1:])), [(t, n) for t, n in zip(T, size)]
+
+
+@pytest.mark.parametrize("N", [1, 64, 512, 1024, 2048, 2049, 3520, 3521, 4096, 4097, 20000, 20481, 32768, 32769])
+def test_norm_workspace_covers_every_smaller_call(N):
+    L = mmvae_amd.lib()
+    size = [L.mmvae_layer_norm_bwd_ws(M, N) for M in [*range(0, 2200), 4096, 4097, 8192, 16384, 16385, 20000, 100000, 1 << 20]]
+    assert all(a <= b for a, b in zip(size, size[1:]))
+
+
 @pytest.mark.parametrize("call", [
     lambda t: ops.layer_norm(t),
     lambda t: ops.layer_norm_backward(t, t, t, t),
