@@ -352,8 +352,11 @@ __global__ __launch_bounds__(BLK, BLK / 256) void k_ln_bwd(NormP a) {
             if constexpr (HOLD) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) w[i] = hw[HOLD ? j : 0][i];
-            } else {  // (a chunk behind the row's end multiplies zeros)
-                lds_get8(lds_anew(lw), slots, c < slots ? c : 0, w);
+            } else {
+                // (a chunk behind the row's end multiplies zeros, by a slot that this thread wrote itself: another wave's
+                // may not be there yet, and what an earlier kernel left in LDS can be a NaN)
+                static_assert(VPT > 1, "the thread's first slot is in the row");
+                lds_get8(lds_anew(lw), slots, c < slots ? c : lane, w);
             }
             if (MASK) {
                 bool on[8] = {true, true, true, true, true, true, true, true};

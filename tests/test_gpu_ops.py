@@ -243,6 +243,25 @@ def test_norm_backward_over_its_inputs(M, N, over):
     assert torch.equal(out, dx) and torch.equal(dw2, dw) and torch.equal(db2, db)
 
 
+@pytest.mark.parametrize("dtype,N,masked", [(BF16, 20000, False), (F16, 16400, False), (BF16, 30000, False), (F32, 20000, False),
+                                            (BF16, 12296, True), (F16, 20000, True), (F32, 8200, True)])
+def test_norm_backward_after_one_that_left_nan_in_lds(dtype, N, masked):
+    """Rows whose weights lie in LDS and whose last chunks leave lanes idle: what such a lane multiplies its zeros with is
+    not what an earlier call (here one with weights of NaN, on every CU) left there."""
+    x, dy, w, b = make(700, N, dtype)
+    kw = dict(p=0.2, seed=3) if masked else {}
+    _, mean, rstd = ops.layer_norm_forward(x, w, b, **kw)
+    nan = torch.full_like(w, float("nan"))
+    want = None
+    for _ in range(4):
+        assert torch.isnan(ops.layer_norm_backward(dy, x, mean, rstd, nan, b, **kw)[0]).all()
+        got = ops.layer_norm_backward(dy, x, mean, rstd, w, b, **kw)
+        assert all(torch.isfinite(t).all() for t in got)
+        assert want is None or all(torch.equal(t, u) for t, u in zip(got, want))
+        want = got
+    check_norm(x[:3], dy[:3], w, b, **kw)
+
+
 def test_norm_leaves_what_is_beside_its_rows():
     """Outputs with a row stride above N: the columns between the rows stay as they were."""
     M, N, ld = 37, 101, 120
