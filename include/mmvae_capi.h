@@ -305,7 +305,7 @@ typedef struct mmvae_norm_args {
     int64_t lddy;
     void *dx;                  /* NULL: not computed */
     int64_t lddx;
-    void *dw, *db;             /* [N] of type wtype (N < 2^26); NULL: not computed */
+    void *dw, *db;             /* [N] of type wtype (N <= 2^26 - 16); NULL: not computed */
     void *ws;                  /* backward with dw or db: mmvae_layer_norm_bwd_ws(M, N) bytes (0: none) */
     int64_t ws_bytes;
     double p;                  /* dropout probability, 0: none */

@@ -875,7 +875,8 @@ const char* norm_check(const mmvae_norm_args& a, bool bwd) {
     }
     if (a.M > 0 && (!a.dy || !a.mean || !a.rstd)) return "dy, mean or rstd is null";
     if (a.dx && !ld_ok(a.lddx, a.N, a.M)) return "dx's row stride is below N";
-    if ((a.dw || a.db) && a.N >= (1 << 26)) return "need N < 2^26 with dw or db";  // (a grid has below 2^32 threads)
+    // (k_ln_wred: 1024 threads for 32 of the 2 x padded width's sums, and a grid has below 2^32 threads)
+    if ((a.dw || a.db) && a.N > (1 << 26) - 16) return "need N <= 2^26 - 16 with dw or db";
     if ((a.dw || a.db) && norm_bwd_ws(a.M, a.N) > 0 && (!a.ws || a.ws_bytes < norm_bwd_ws(a.M, a.N)))
         return "the workspace is below mmvae_layer_norm_bwd_ws(M, N) bytes";
     return nullptr;

@@ -193,6 +193,18 @@ def test_norm_no_rows_and_parts():
         assert torch.equal(part[k], all3[k]) and all(part[i] is None for i in range(3) if i != k)
 
 
+def test_norm_weight_gradients_of_the_widest_rows():
+    """No rows of the largest width that is taken: its last launch has the most threads, and clears both sums."""
+    N = 2 ** 26 - 16
+    x, st = torch.empty(0, N, device=DEV), torch.empty(0, device=DEV)
+    w = torch.ones(N, device=DEV)
+    dx, dw, db = ops.layer_norm_backward(x, x, st, st, w)
+    assert dx.shape == (0, N) and not dw.any() and not db.any()
+    with pytest.raises(mmvae_amd.MMVAEError, match="2\\^26 - 16"):
+        x = torch.empty(0, N + 1, device=DEV)
+        ops.layer_norm_backward(x, x, st, st)
+
+
 def test_norm_equal_calls_equal_bits():
     x, dy, w, b = make(3000, 300, F32)
     one = check_norm(x, dy, w, b, p=0.2, seed=1)

@@ -82,6 +82,16 @@ def test_norm_backward_refuses(kw):
     assert mmvae_amd.lib().mmvae_layer_norm_bwd(pack_norm(**kw)) == -1
 
 
+@pytest.mark.parametrize("N", [2 ** 26 - 15, 2 ** 26 - 8, 2 ** 26 - 7, 2 ** 26 - 1, 2 ** 26])
+@pytest.mark.parametrize("kw", [dict(M=0), dict(M=1), dict(M=600, ldx=0, lddy=0, dx=0), dict(db=0), dict(dw=0)])
+def test_norm_backward_refuses_widths_whose_padded_sums_pass_the_grid(N, kw):
+    """The weight gradients' last launch has 1024 threads for 32 of the sums of twice the width, padded to 8: 2^32 from
+    N = 2^26 - 15 on."""
+    L = mmvae_amd.lib()
+    assert L.mmvae_layer_norm_bwd(pack_norm(N=N, lddx=N, ws_bytes=1 << 50, **kw)) == -1
+    assert b"2^26 - 16" in L.mmvae_last_error(None)
+
+
 @pytest.mark.parametrize("kw", [dict(M=-1), dict(N=-1), dict(N=2 ** 31), dict(dtype=5), dict(p=-1.0), dict(p=2.0), dict(p=float("nan")), dict(x=0),
                                 dict(y=0), dict(ldx=-8), dict(ldy=7), dict(N=1 << 24, ldx=1 << 24, ldy=1 << 24), dict(x=4097, dtype=1),
                                 dict(M=1 << 20, N=1 << 18, ldy=1 << 18)])
