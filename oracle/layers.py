@@ -51,6 +51,13 @@ def norm(x, w, b, eps, factor, relu):
     return y, mean[:, 0], rstd[:, 0], u
 
 
+def column_chain(M, N):
+    """Additions in a column's sum over M rows, with room.  In strips: a thread's rows (M / 512, or up to 4), 6 lane steps, 8
+    waves; in parts: a thread's rows (M / 256 at most), 32 row groups, a stage of 16 and one of 32; of rows that may be read
+    in sweeps: 128 stripes of rows and two stages."""
+    return M / (128 if N > 20480 else 256) + 96
+
+
 def norm_grads(dy, x, w, eps, factor, mask):
     """dx, dw, db and the error bounds of their 32-bit evaluation (before the final rounding), with the ReLU's mask."""
     M, N = x.shape
@@ -67,12 +74,12 @@ def norm_grads(dy, x, w, eps, factor, mask):
     ag = (g.abs() * a).mean(1, keepdim=True)
     bdx = ROW * U32 * rstd * (2 * g.abs() + 2 * g.abs().mean(1, keepdim=True) + 2 * a * (g * xh).abs().mean(1, keepdim=True) + xh.abs() * 2 * ag)
     dw, db = (du * xh).sum(0), du.sum(0)
-    # A column's sums: at most M / 256 + 96 additions (a thread's rows, the workgroup's, the partial rows')
-    col = M / 256 + 96
+    col = column_chain(M, N)
     return dx, dw, db, bdx, U32 * ((col + ROW) * (du.abs() * a).sum(0)), U32 * col * du.abs().sum(0)
 
 
-# additions in a row's sum: a thread's 8 x 4 elements, 6 lane steps, 16 waves; in sweeps (N > 32768) 8 + N / 8192
+# Additions in a row's sum, with room: 8 elements of a chunk, a thread's up to 8 chunks, 6 lane steps, 8 waves; in sweeps
+# (N > 32768) 8 + N / 8192 + 6 + 16.  The backward's two sums are chains of up to 8 x 8 + 14: the 2 in bdx covers them.
 ROW = 72
 
 
@@ -91,15 +98,42 @@ def embedding(ids, table, scale, add=None):
     return y if add is None else y + add
 
 
+def embedding_chain(T, N, rows):
+    """Additions from a token's dy to its row of the gradient: its group's tokens, the piece's groups, a share of the pieces
+    and the shares.  gb groups of tg tokens are a piece; 8, 16 or 32 lanes a row of N."""
+    nc = (N + 7) // 8
+    lanes = 8 if nc <= 8 else 16 if 5 * (-(-nc // 32) * 32) > 6 * (-(-nc // 16) * 16) else 32
+    gb = 256 // lanes
+    tg = 8 if T <= 32768 else 512 // gb if rows <= 64 else 16
+    return tg + gb + -(-T // (gb * tg)) // gb + 1 + gb
+
+
+def longest_chain(T, gb, tg, few):
+    """dy of T tokens of one id whose 32-bit sum loses nearly half a step of 1 in every addition: 1, then addends just below
+    2^-24 along one chain (sorted: a share of the pieces behind the first; few rows: a group, its piece, a share, the shares)."""
+    d, P = torch.zeros(T), gb * tg
+    tiny = 0.999 * U32
+    if few:
+        d[1:tg] = tiny
+        d[tg:P:tg] = tiny
+        d[P:gb * P:P] = tiny
+        d[gb * P::gb * P] = tiny
+        d[0] = 1
+    else:
+        d[P + gb * P::gb * P] = tiny
+        d[P] = 1
+    return d
+
+
 def embedding_grad(dy, ids, rows, scale):
-    """The table's gradient and the bound of its 32-bit sum: chains of at most 128 additions (32 of a group,
-    32 groups, the pieces of a run and their groups), the scale's rounding."""
+    """The table's gradient and the bound of its 32-bit sum: n additions and the scale's rounding, (1 + u)^(n + 1) - 1."""
     ok = (ids >= 0) & (ids < rows)
     i = torch.where(ok, ids, rows).reshape(-1).long()
     d = dy.reshape(-1, dy.shape[-1])
     out = torch.zeros(rows + 1, d.shape[1]).double().index_add_(0, i, d)
     mag = torch.zeros(rows + 1, d.shape[1]).double().index_add_(0, i, d.abs())
-    return out[:rows] * scale, 130 * U32 * abs(scale) * mag[:rows]
+    n = embedding_chain(d.shape[0], d.shape[1], rows) + 1
+    return out[:rows] * scale, n * U32 / (1 - n * U32) * abs(scale) * mag[:rows]
 
 
 # ---- the models with normalised, dropped-out, label-conditioned layer chains --------------------

@@ -388,6 +388,17 @@ def test_embedding_many_tiles(T, V):
     check_embedding(tokens(T, V, True), V, 9, F32)
 
 
+@pytest.mark.parametrize("N,V,gb,tg", [(136, 300, 8, 16), (256, 12, 8, 64)])
+def test_embedding_hot_id_of_many_tokens(N, V, gb, tg):
+    """262144 tokens of one id, whose sum loses nearly half a step with each addition of its longest chain, and random ones."""
+    T = 262144
+    ids = torch.full((T,), V - 1, device=DEV)
+    for col in (layers.longest_chain(T, gb, tg, V <= 64), torch.randn(T, generator=torch.Generator().manual_seed(N))):
+        d = ops.embedding_backward(col[:, None].to(DEV).expand(T, N), ids, V)
+        D, bound = layers.embedding_grad(col[:, None].double().expand(T, N), ids.cpu(), V, 1.0)
+        close(d, D, bound, "dtable")
+
+
 def test_embedding_id_types_shapes_add():
     ids = tokens(600, 50, True)
     a = check_embedding(ids, 50, 40, F32, add=True)

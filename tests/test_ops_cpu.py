@@ -133,6 +133,46 @@ def test_workspace_sizes_grow_with_the_call():
         assert L.mmvae_embedding_bwd_ws(T, 33, 7) >= 7 * 4 * 40  # few rows: a partial of each
 
 
+def sums_as_the_kernels(d, gb, tg, few):
+    """One id's tokens in the kernels' order and in float32: groups, pieces, shares of the pieces."""
+    d = d.numpy().reshape(-1, gb, tg)
+    g = np.zeros(d.shape[:2], np.float32)
+    for k in range(tg):
+        g += d[:, :, k]
+    p = np.zeros(len(g), np.float32)
+    for k in range(gb):
+        p += g[:, k]
+    first, rest = (np.float32(0), p) if few else (p[0], p[1:])
+    shares = np.zeros(gb, np.float32)
+    for j, v in enumerate(rest):
+        shares[j % gb] += v
+    for v in shares:
+        first = np.float32(first + v)
+    return float(first)
+
+
+@pytest.mark.parametrize("T,N,V,gb,tg", [(262144, 136, 300, 8, 16), (262144, 256, 12, 8, 64), (262144, 600, 2, 8, 64), (1 << 20, 256, 70, 8, 16),
+                                         (32768, 136, 70, 8, 8), (262144, 128, 70, 16, 16)])
+def test_oracle_embedding_bound_holds_for_the_longest_chains(T, N, V, gb, tg):
+    """Sums in the kernels' order that lose nearly half a step with every addition of one chain stay within the bound."""
+    d = layers.longest_chain(T, gb, tg, V <= 64)
+    want, bound = layers.embedding_grad(d[:, None].double().expand(T, N), torch.ones(T, dtype=torch.int64), V, 1.0)
+    off = abs(sums_as_the_kernels(d, gb, tg, V <= 64) - float(want[1, 0]))
+    assert off <= float(bound[1, 0]), (off / layers.U32, float(bound[1, 0]) / layers.U32)
+    assert off >= 0.9 * float(bound[1, 0]) - (2 * gb + tg) * layers.U32  # (the bound is no larger than such sums need)
+
+
+@pytest.mark.parametrize("M", [20000, 65536, 1 << 20])
+def test_oracle_column_bound_holds_for_rows_in_sweeps(M):
+    """A stripe takes every 128th row: 1 and addends just below half a step of it, each lost."""
+    s = np.float32(1)
+    for _ in range(M // 128 - 1):
+        s += np.float32(0.999 * layers.U32)
+    off = (M // 128 - 1) * 0.999 * layers.U32 + 1 - float(s)
+    assert off <= layers.column_chain(M, 40000) * layers.U32
+    assert M < 65536 or off > layers.column_chain(M, 20000) * layers.U32  # (those of other rows are shorter)
+
+
 @pytest.mark.parametrize("N", [1, 24, 64, 128, 136, 517, 1025])  # 8, 16 and 32 lanes a row
 @pytest.mark.parametrize("V", [1, 5, 12, 64, 65, 300, 30000])
 def test_embedding_workspace_covers_every_smaller_call(V, N):
