@@ -399,6 +399,21 @@ def test_embedding_hot_id_of_many_tokens(N, V, gb, tg):
         close(d, D, bound, "dtable")
 
 
+@pytest.mark.parametrize("T,V,N", [(300, 5, 40), (5000, 300, 130), (33000, 12, 24)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_embedding_gradient_of_strided_and_repeated_rows(T, V, N, dtype):
+    """dy inside wider rows, with a column stride, transposed, one row for all tokens, one value for all."""
+    g = torch.Generator().manual_seed(T)
+    ids = tokens(T, V, True)
+    wide = torch.randn(T, 2 * N + 3, generator=g).to(dtype).to(DEV)
+    for dy in (wide[:, 3:N + 3], wide[:, 1:2 * N + 1:2], wide[:, :N].t().contiguous().t(), wide[:1, :N].expand(T, N), wide[:1, :1].expand(T, N),
+               wide[:, :1].expand(T, N)):
+        d = ops.embedding_backward(dy, ids, V, 0.5)
+        D, bound = layers.embedding_grad(cpu64(dy), ids.cpu(), V, 0.5)
+        close(d, D, bound, "dtable")
+        assert torch.equal(d, ops.embedding_backward(dy.contiguous(), ids, V, 0.5))
+
+
 def test_embedding_id_types_shapes_add():
     ids = tokens(600, 50, True)
     a = check_embedding(ids, 50, 40, F32, add=True)
