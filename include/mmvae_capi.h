@@ -66,6 +66,9 @@ typedef struct mmvae_cfg {
     float grad_clip;     /* clip_grad_norm_ max norm, mmvae_alg.hh:308 (always 1.0 there: Q7) */
     float kappa_min;     /* vMF --kappa_min (vmf.hh:61) */
     float kappa_max;     /* vMF --kappa_max (vmf.hh:62) */
+    uint32_t size;       /* set by mmvae_cfg_default: bytes of the cfg that program and library both know.  With any
+                            other value (it was padding in older headers) the cfg ends behind dec_hidden, and the
+                            fields from layer_norm on count as their defaults. */
     uint64_t seed;       /* Philox seed for the reparameterisation noise when none is injected */
     int32_t relu;        /* --relu: NB ReLU after each frozen encoder / hidden decoder Linear
                             (nb.hh:336-346, 372-373); vMF after each Angular encoder / hidden
@@ -95,8 +98,12 @@ typedef struct mmvae_cfg {
     int32_t reserved;
 } mmvae_cfg;
 
-/* Fill a cfg with the reference defaults (mmvae_alg.hh:19-23, nb.hh:58-61, vmf.hh:59-63). */
+/* Fill a cfg with the reference defaults (mmvae_alg.hh:19-23, nb.hh:58-61, vmf.hh:59-63).  A program says how
+ * large its cfg is; the symbol mmvae_cfg_default, which programs built with older headers call, writes no field
+ * behind dec_hidden. */
 void mmvae_cfg_default(mmvae_cfg* cfg, int32_t model);
+void mmvae_cfg_default_n(mmvae_cfg* cfg, uint64_t bytes, int32_t model);
+#define mmvae_cfg_default(cfg, model) mmvae_cfg_default_n((cfg), sizeof(mmvae_cfg), (model))
 
 /* Create an engine on HIP device `device`.  Replaces constructing nbvae_t / vmf_vae_t
  * (nb.hh:299-401, vmf.hh:307-389) plus the torch::optim::Adam of mmvae_alg.hh:234-237.

@@ -253,28 +253,42 @@ static void use_slot(Engine* e, int s) {
 
 extern "C" {
 
-void mmvae_cfg_default(mmvae_cfg* c, int32_t model) {
-    std::memset(c, 0, sizeof(*c));
-    c->model = model;
-    c->dtype = MMVAE_DTYPE_F32;
-    c->C = 1;
-    c->K = 2;   // --mean_latent / --latent default (nb.hh:59, vmf.hh:60)
-    c->H = 1;
-    c->R = 1;
-    c->max_batch = 100;  // --batch_size default (mmvae.hh:35)
-    c->lr = 1e-3f;
-    c->weight_decay = 1e-4f;
-    c->grad_clip = 1.f;
-    c->kappa_min = 0.1f;
-    c->kappa_max = 10.f;
-    c->seed = 42;
-    c->label_scale = 1.f;
+// what a cfg of a header without the layer options holds
+static constexpr size_t CFG_OLD = offsetof(mmvae_cfg, layer_norm);
+static_assert(sizeof(mmvae_cfg) == 256 && offsetof(mmvae_cfg, size) == 76 && offsetof(mmvae_cfg, seed) == 80 && CFG_OLD == 228,
+              "the older fields stay where they were");
+
+void mmvae_cfg_default_n(mmvae_cfg* out, uint64_t bytes, int32_t model) {
+    mmvae_cfg c;
+    std::memset(&c, 0, sizeof(c));
+    c.model = model;
+    c.dtype = MMVAE_DTYPE_F32;
+    c.C = 1;
+    c.K = 2;   // --mean_latent / --latent default (nb.hh:59, vmf.hh:60)
+    c.H = 1;
+    c.R = 1;
+    c.max_batch = 100;  // --batch_size default (mmvae.hh:35)
+    c.lr = 1e-3f;
+    c.weight_decay = 1e-4f;
+    c.grad_clip = 1.f;
+    c.kappa_min = 0.1f;
+    c.kappa_max = 10.f;
+    c.seed = 42;
+    c.label_scale = 1.f;
+    const bool whole = bytes >= sizeof(c);
+    c.size = whole ? (uint32_t)sizeof(c) : 0;
+    std::memcpy(out, &c, whole ? sizeof(c) : CFG_OLD);
 }
+void (mmvae_cfg_default)(mmvae_cfg* c, int32_t model) { mmvae_cfg_default_n(c, CFG_OLD, model); }
 
 const char* mmvae_last_error(mmvae_h h) { return h ? h->err.c_str() : g_last_error.c_str(); }
 
-int mmvae_create(const mmvae_cfg* cfg, int device, mmvae_h* out) {
-    if (!cfg || !out) FAIL((Engine*)nullptr, MMVAE_E_ARG, "null cfg/out");
+int mmvae_create(const mmvae_cfg* cfg_in, int device, mmvae_h* out) {
+    if (!cfg_in || !out) FAIL((Engine*)nullptr, MMVAE_E_ARG, "null cfg/out");
+    mmvae_cfg whole;
+    mmvae_cfg_default(&whole, cfg_in->model);
+    std::memcpy(&whole, cfg_in, cfg_in->size == sizeof(whole) ? sizeof(whole) : CFG_OLD);
+    const mmvae_cfg* const cfg = &whole;
     if (cfg->model != MMVAE_MODEL_NB && cfg->model != MMVAE_MODEL_VMF)
         FAIL((Engine*)nullptr, MMVAE_E_ARG, "model must be MMVAE_MODEL_NB or MMVAE_MODEL_VMF");
     if (cfg->model == MMVAE_MODEL_VMF && !(cfg->kappa_min > 0.f && cfg->kappa_max >= cfg->kappa_min))

@@ -35,7 +35,7 @@ class Cfg(ctypes.Structure):
     _fields_ = [("model", ctypes.c_int32), ("dtype", ctypes.c_int32), ("D", ctypes.c_int64),
                 ("C", ctypes.c_int64), ("K", ctypes.c_int64), ("H", ctypes.c_int64), ("R", ctypes.c_int64),
                 ("max_batch", ctypes.c_int64), ("lr", ctypes.c_float), ("weight_decay", ctypes.c_float),
-                ("grad_clip", ctypes.c_float), ("kappa_min", ctypes.c_float), ("kappa_max", ctypes.c_float),
+                ("grad_clip", ctypes.c_float), ("kappa_min", ctypes.c_float), ("kappa_max", ctypes.c_float), ("size", ctypes.c_uint32),
                 ("seed", ctypes.c_uint64), ("relu", ctypes.c_int32), ("n_enc_hidden", ctypes.c_int32),
                 ("n_dec_hidden", ctypes.c_int32), ("enc_hidden", ctypes.c_int32 * MAX_HIDDEN),
                 ("dec_hidden", ctypes.c_int32 * MAX_HIDDEN), ("layer_norm", ctypes.c_int32), ("dropout", ctypes.c_float),
@@ -64,6 +64,7 @@ def lib():
     i64, i32, f32p, i64p = ctypes.c_int64, ctypes.c_int32, ctypes.POINTER(ctypes.c_float), ctypes.POINTER(ctypes.c_int64)
     sig = {
         "mmvae_cfg_default": (None, [ctypes.POINTER(Cfg), i32]),
+        "mmvae_cfg_default_n": (None, [ctypes.POINTER(Cfg), ctypes.c_uint64, i32]),
         "mmvae_create": (ctypes.c_int, [ctypes.POINTER(Cfg), ctypes.c_int, ctypes.POINTER(h)]),
         "mmvae_destroy": (ctypes.c_int, [h]),
         "mmvae_last_error": (ctypes.c_char_p, [h]),
@@ -122,7 +123,7 @@ def lib():
 
 def default_cfg(model=MODEL_NB):
     c = Cfg()
-    lib().mmvae_cfg_default(ctypes.byref(c), model)
+    lib().mmvae_cfg_default_n(ctypes.byref(c), ctypes.sizeof(c), model)
     return c
 
 

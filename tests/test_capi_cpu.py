@@ -4,6 +4,7 @@ failure without a GPU) behave — no compute calls."""
 import ctypes
 import os
 import re
+import subprocess
 
 import numpy as np
 import pytest
@@ -193,3 +194,56 @@ def test_graph_key_uneven_slices_refused_before_any_collective(graph_key_probe, 
     assert any(r[1] == -1 for r in rows), rows
     assert all(r[1] == -1 or r[2] * world == n_total for r in rows)
     assert all(r[1] == 0 for r in graph_key_probe(world, n_total, False))
+
+
+OLDER_CLIENT = r"""
+#include <stdint.h>
+#include <stdio.h>
+#include <string.h>
+struct cfg {  /* mmvae_cfg as it was before the layer options */
+    int32_t model, dtype;
+    int64_t D, C, K, H, R, max_batch;
+    float lr, weight_decay, grad_clip, kappa_min, kappa_max;
+    uint64_t seed;
+    int32_t relu, n_enc_hidden, n_dec_hidden, enc_hidden[16], dec_hidden[16];
+};
+void mmvae_cfg_default(struct cfg*, int32_t);
+int mmvae_create(const struct cfg*, int, void**);
+const char* mmvae_last_error(void*);
+int main(void) {
+    struct { struct cfg c; unsigned char behind[64]; } s;
+    void* h;
+    int i, touched = 0;
+    memset(&s, 0xff, sizeof(s));  /* (as floats: NaN, which the layer options refuse) */
+    mmvae_cfg_default(&s.c, 0);
+    for (i = 0; i < 64; ++i) touched += s.behind[i] != 0xff;
+    s.c.D = 10;
+    i = mmvae_create(&s.c, 99, &h);
+    printf("%d %d %d %g|%s\n", touched, i, (int)s.c.max_batch, s.c.kappa_max, mmvae_last_error(0));
+    memset((char*)&s.c + 76, 0xff, 4);  /* a cfg filled by hand: its padding holds anything */
+    i = mmvae_create(&s.c, 99, &h);
+    printf("%d|%s\n", i, mmvae_last_error(0));
+    return 0;
+}
+"""
+
+
+def test_programs_built_before_the_layer_options(tmp_path):
+    """Their cfg ends at dec_hidden: nothing behind it is written or read."""
+    c = tmp_path / "older.c"
+    c.write_text(OLDER_CLIENT)
+    subprocess.run(["gcc", str(c), "-o", str(tmp_path / "older"), mmvae_amd.LIB_PATH, "-Wl,-rpath," + os.path.dirname(mmvae_amd.LIB_PATH),
+                    "-Wl,--allow-shlib-undefined"], check=True)
+    out = subprocess.run([str(tmp_path / "older")], check=True, capture_output=True, text=True).stdout.splitlines()
+    assert out == ["0 -2 100 10|no HIP device 99", "-2|no HIP device 99"]
+
+
+def test_cfg_carries_its_size():
+    """Through the header and the binding a cfg holds its size, and the layer options count."""
+    c = mmvae_amd.default_cfg(mmvae_amd.MODEL_NB)
+    assert c.size == ctypes.sizeof(c) and c.label_scale == 1.0
+    h, L = ctypes.c_void_p(), mmvae_amd.lib()
+    c.D, c.dropout = 10, 2.0
+    assert L.mmvae_create(ctypes.byref(c), 99, ctypes.byref(h)) == -1 and b"dropout" in L.mmvae_last_error(None)
+    c.dropout, c.n_labels = 0.5, -1
+    assert L.mmvae_create(ctypes.byref(c), 99, ctypes.byref(h)) == -1 and b"n_labels" in L.mmvae_last_error(None)
