@@ -38,7 +38,20 @@ static bool file_exists(const std::string& f) {
     return !f.empty() && stat(f.c_str(), &st) == 0;
 }
 
-int parse_options(int argc, const char** argv, int model, CliOptions& o) {
+int parse_options(int argc, const char** argv_in, int model, CliOptions& o) {
+    // "--label_scale -1e2" as one word: the groups that do not know the option would read the negative number as
+    // short options (-e 2)
+    std::vector<std::string> words;
+    for (int i = 0; i < argc; ++i) {
+        const std::string w = argv_in[i];
+        const bool scale = w.size() > std::strlen("--label_") && std::string("--label_scale").compare(0, w.size(), w) == 0;
+        words.push_back(scale && i + 1 < argc ? w + "=" + argv_in[++i] : w);
+    }
+    std::vector<const char*> args;
+    for (const std::string& w : words) args.push_back(w.c_str());
+    argc = (int)args.size();
+    args.push_back(nullptr);
+    const char** const argv = args.data();
     // the reference's three option groups through the drop-in parsers (include/mmvae/options.hh)
     mmvae_options_t mo;
     bool help = false;

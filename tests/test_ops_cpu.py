@@ -302,3 +302,40 @@ def test_cli_layer_options_refused(tmp_path, exe):
                       (["--labels", str(lab)], "1 labels for 2"), (["--labels", str(tmp_path / "none")], "cannot read")):
         r = subprocess.run(base + more, capture_output=True, text=True, timeout=60)
         assert r.returncode == 1 and msg in r.stderr, (more, r.stderr)
+
+
+PARSE = r"""
+#include <cstdio>
+#include "cli.hh"
+using namespace mmvae_host;
+int main(int argc, const char** argv) {
+    CliOptions o;
+    const int rc = parse_options(argc, argv, argv[1][0] - '0', o);
+    std::printf("%d %g %g %lld %lld %lld %lld %zu %s\n", rc, o.label_scale, o.dropout, (long long)o.H, (long long)o.R, (long long)o.latent,
+                (long long)o.train.max_epoch, o.enc_layers.size(), o.labels.c_str());
+    return 0;
+}
+"""
+
+
+@pytest.mark.parametrize("model", ["0", "1"])
+def test_cli_negative_label_scale_is_no_short_option(tmp_path, model):
+    """A negative scale with an exponent reads as a scale, and nothing of it as another group's short options."""
+    src, exe, lib = tmp_path / "p.cc", tmp_path / "p", os.path.dirname(mmvae_amd.LIB_PATH)
+    src.write_text(PARSE)
+    subprocess.run(["g++", "-std=c++17", str(src), "-o", str(exe), "-I", os.path.join(lib, "..", "host"), "-L" + lib, "-lmmvae_host", "-lmmvae",
+                    "-Wl,-rpath," + lib], check=True)
+    x = tmp_path / "x.mtx"
+    x.write_text("")
+
+    def parsed(*more):
+        r = subprocess.run([str(exe), model, "--mtx", str(x), "--out", "o", *more], capture_output=True, text=True, check=True).stdout.split()
+        return r[:2], r[2:]
+    base = parsed("--labels", "f")
+    assert base[0] == ["0", "1"]
+    for v in ("-1e2", "-1E2", "-0.5", "-2e-3", "-1e+1", "3"):
+        for name in ("--label_scale", "--label_sc"):
+            for words in ((name, v), (f"{name}={v}",)):
+                rc, rest = parsed(*words, "--labels", "f")
+                assert rc == ["0", f"{float(v):g}"] and rest == base[1], (words, rc, rest)
+    assert parsed("--label_scale")[0] == ["0", "1"]  # (no value: ignored, as all options are)
