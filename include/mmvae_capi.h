@@ -333,7 +333,7 @@ int64_t mmvae_layer_norm_bwd_ws(int64_t M, int64_t N);
 /* y[r][c] = x[r][c] times its dropout factor; a dropped element is 0 whatever x holds.  The
  * gradient is the same call on dy.  y may be x. */
 typedef struct mmvae_dropout_args {
-    int64_t M, N;
+    int64_t M, N;              /* rows (< 2^31 - 65536), columns (< 2^24); M N < 2^37 */
     const void *x;
     int64_t ldx;
     void *y;
@@ -351,7 +351,7 @@ int mmvae_dropout(const mmvae_dropout_args* args);
  * zeros and has no gradient.  Backward: dtable[v] = scale sum of dy[t] over ids[t] = v, every row
  * of [V][N] written (contiguous, 4-byte aligned), the tokens summed in a fixed order. */
 typedef struct mmvae_embedding_args {
-    int64_t T, N, V;           /* tokens, width (< 2^24), table rows; T, V < 2^31 - 65536 */
+    int64_t T, N, V;           /* tokens, width (< 2^24), table rows; T, V < 2^31 - 65536, T N < 2^37 */
     const void *ids;           /* [T] int64 (ids64 != 0) or int32 */
     const void *table;         /* forward */
     int64_t ldt;

@@ -59,16 +59,17 @@ template <class T> MMVAE_DEV void ldws(const void* w, bool f32, int col, int n, 
     for (int i = 0; i < 8; ++i) v[i] *= s;
 }
 
-// How a thread keeps its row and weights, by the registers that a wave has (256 at 512 threads, 128 at
-// 1024; with fewer threads a row other rows' waves hide the loads too):
+// How a thread keeps its row and weights, by the 256 registers that a wave has at up to 512 threads (with fewer
+// threads a row other rows' waves hide the loads too):
 //   HOLD  the weights in registers over all rows, else in LDS (16 V of w and b forward, 8 V of w backward);
 //   PRE   the next row's loads in flight under this row's sums;
 //   AGAIN (backward) x and dy read in both phases, where they do not fit beside the 16 V column sums.
 // ROOM: what is left beside temporaries, as the compiler uses them (no variant that is launched spills
 // more than a few registers).
 template <class T, int VPT, int BLK, bool MASK, bool EVEN> struct LnKeep {
+    static_assert(BLK <= 512, "256 registers a lane");
     static constexpr int X = (int)sizeof(T) * 2;  // registers of a chunk
-    static constexpr int ROOM = (BLK >= 1024 ? 128 : 256) - 66 - (MASK ? 10 : 0) - (EVEN ? 0 : 14);
+    static constexpr int ROOM = 256 - 66 - (MASK ? 10 : 0) - (EVEN ? 0 : 14);
     static constexpr int B = 16 + (MASK ? 12 : 0);  // a chunk's column sums (and masks)
     static constexpr bool F_HOLD = (16 + X) * VPT <= ROOM;
     static constexpr bool F_PRE = ((F_HOLD ? 16 : 0) + 2 * X) * VPT <= ROOM;
@@ -502,7 +503,8 @@ __global__ __launch_bounds__(1024) void k_ln_wred(int N, int64_t Np, int G, cons
 }
 
 // Rows too long for the registers (N > 32,768): each sweep reads the row again, from the last-level cache
-// where it fits (2048 x 40000 bf16: forward 109 us, 3.0 TB/s of x and y; backward 238 us)
+// where it fits (2048 x 40000 bf16: forward 104 us, 3.1 TB/s of x and y; backward 235 us).  32768 / 32776 columns
+// of 4096 bf16 rows: forward 100 / 187 us, backward 264 / 385.
 static constexpr int LONG_N = 32768;
 template <class T> __global__ __launch_bounds__(1024) void k_ln_fwd_long(NormP a) {
     __shared__ float red[2][16];
@@ -663,7 +665,9 @@ constexpr int HALF_N = 3520;
 template <class F> inline hipError_t by_width_bwd(int N, F&& f) {
     return N > HALF_N && N <= 4096 ? f(I<512>{}, I<1>{}, I<512>{}) : by_width(N, f);
 }
-// (backward with masks: above 20,480 columns the sums do not stay in the registers, 228 bytes a lane spilled)
+// Backward with masks: above 20,480 columns the sums do not stay in the registers (228 bytes a lane spilled), and the
+// rows are read in sweeps.  Dropout, us, 20480 / 20488 columns: 100 rows bf16 14.9 / 18.3, 512 36 / 40, 2048 92 / 125, 4096
+// 145 / 264 (f32 262 / 415); without masks 4096 rows 127 / 133.
 constexpr int LONG_PARTS = 128, FITS_N = 20480, STRIP_N = 4096;
 // A backward of few rows sums dw and db in strips of columns, beside the row workgroups of the same launch: x
 // and dy are read a second time, but there are no partial sums to write, read and add up.  us of both ways

@@ -132,7 +132,7 @@ template <class T> __global__ __launch_bounds__(256) void k_emb_fwd(EmbF a) {
 // 128 f32: 5.8 + 3.4.
 // =======================================================================================
 static constexpr int FEW = 64;      // (128 columns bf16, 64 rows against 65 sorted: 256 tokens 8.2 / 12.2 us, 4096
-                                    // 8.9 / 15.3, 32768 16.2 / 18.3, 262144 30.5 / 28.9)
+                                    // 8.9 / 15.3, 32768 16.2 / 18.3, 262144 30.5 / 28.9: level from there, whatever T)
 static constexpr int RTHR = 1024;   // a sort tile: 16 waves x KPT x 64 tokens
 static constexpr int RONE = 4096;   // tokens that one workgroup sorts, KPT = 4 (4096 tokens into 20000 x 128 bf16
                                     // 19.4 us, 4097 in tiles 24.9)

@@ -28,7 +28,8 @@ from . import _ops  # noqa: E402
 
 _ops.set_error(MMVAEError)
 
-# the C argument structs, member by member (8-byte members first: no padding)
+# the C argument structs, member by member (8-byte members first: no padding), for calls of the C entries through
+# lib(): lib().mmvae_dropout(DROPOUT_ARGS.pack(...)); the calls below go through _ops
 NORM_ARGS = struct.Struct("=2q Q q 2Q Q q 2Q Q q Q q 2Q Q q d 3Q Q Q 3i f 2i")
 DROPOUT_ARGS = struct.Struct("=2q Q q Q q d 3Q Q Q 2i")
 EMBEDDING_ARGS = struct.Struct("=3q 2Q q Q q Q q Q q Q Q q Q 3i f")
