@@ -41,6 +41,10 @@ class Cfg(ctypes.Structure):
                 ("dec_hidden", ctypes.c_int32 * MAX_HIDDEN), ("layer_norm", ctypes.c_int32), ("dropout", ctypes.c_float),
                 ("n_labels", ctypes.c_int64), ("label_scale", ctypes.c_float), ("reserved", ctypes.c_int32)]
 
+    def __init__(self, *args, **kw):
+        super().__init__(*args, **kw)
+        self.size = ctypes.sizeof(self)  # (a cfg without it has no fields behind dec_hidden)
+
 
 class StepArgs(ctypes.Structure):
     _fields_ = [("cell_ids", ctypes.POINTER(ctypes.c_int64)), ("ridx", ctypes.POINTER(ctypes.c_int64)),

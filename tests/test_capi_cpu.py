@@ -242,6 +242,7 @@ def test_cfg_carries_its_size():
     """Through the header and the binding a cfg holds its size, and the layer options count."""
     c = mmvae_amd.default_cfg(mmvae_amd.MODEL_NB)
     assert c.size == ctypes.sizeof(c) and c.label_scale == 1.0
+    assert mmvae_amd.Cfg().size == ctypes.sizeof(c)  # (one filled by hand too)
     h, L = ctypes.c_void_p(), mmvae_amd.lib()
     c.D, c.dropout = 10, 2.0
     assert L.mmvae_create(ctypes.byref(c), 99, ctypes.byref(h)) == -1 and b"dropout" in L.mmvae_last_error(None)
