@@ -162,6 +162,39 @@ def test_norm_offset_rows():
     assert torch.equal(y[4], b) and torch.isfinite(dx).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("off", [0.0, 300.0, -20000.0])
+@pytest.mark.parametrize("M,N", [(300, 48), (2500, 128), (40, 500), (600, 1000), (700, 2049), (1100, 4096), (600, 5000), (60, 16400), (40, 20488), (600, 33000)])
+def test_norm_relu_takes_one_side_in_both_directions(M, N, off, dtype):
+    """With dy = 1 the bias's gradient counts the rows whose y is above 0: the backward's u is the forward's to the bit, also
+    where the mean is far above the spread and u near 0 is all rounding."""
+    x, dy, w, b = make(M, N, F32)
+    x = (3 * x + off).to(dtype)
+    w, b = w.clamp(min=0.1), 0.01 * b
+    y, mean, rstd = ops.layer_norm_forward(x, w, b, relu=True)
+    _, _, db = ops.layer_norm_backward(torch.ones_like(x), x, mean, rstd, w, b, relu=True, need=(False, False, True))
+    more = cpu64(db - (y > 0).sum(0))
+    if dtype == F16:  # (u up to 2^-25 rounds to 0: as many rows more as have such a u within its error)
+        X, W, B = cpu64(x), cpu64(w), cpu64(b)
+        near = (layers.norm(X, W, B, 1e-5, 1.0, False)[3].abs() <= layers.norm_bound(X, W, B, 1e-5, 1.0) + 2.0 ** -25) & (y == 0).cpu()
+        assert (more >= 0).all() and (more <= near.sum(0)).all()
+    else:
+        assert not more.any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N", [7, 48, 500, 2049, 12000, 33000])
+def test_norm_of_constant_rows_is_the_bias(N, dtype):
+    """Rows of one value whose sum is exact in 32 bits: in f32 the mean is that value and y the bias."""
+    x = torch.tensor([1.0, -3.0, 0.5, 100.0, 0.0], device=DEV).to(dtype)[:, None].expand(5, N).contiguous()
+    _, dy, w, b = make(5, N, dtype)
+    y, mean, rstd = ops.layer_norm_forward(x, w, b)
+    if dtype == F32:
+        assert torch.equal(mean, x[:, 0]) and torch.equal(y, b.expand(5, N))
+    assert torch.equal(y[4], b.to(dtype))  # (16 bits: xh = x r - m r is off by the product's rounding where the row is not 0)
+    check_norm(x, dy, w, b)
+
+
 def test_norm_infinities_stay_in_their_rows():
     x, dy, w, b = make(40, 500, F32)
     clean = ops.layer_norm_forward(x, w, b)
