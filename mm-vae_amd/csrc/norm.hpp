@@ -40,21 +40,19 @@ struct NormP {
 };
 
 // A row's statistics, and xh and u = xh w + b as forward and backward both compute them (the ReLU's side
-// must be the same).  f32: xh from the difference, exact near the mean; 16-bit values carry 2^-9 and more
-// themselves: one fma.  w and b come multiplied by the dropout factor (a ReLU commutes with it).
-// f32: the mean is a quotient.  A product, sum (1 / N), goes into the difference unrounded (one fma), and the
-// forward's u is then not that of the stored mean; and a row of one value has a difference of 0 (no time lost: 65536
-// x 128 f32 11.7 us, 4096 x 128 with dropout 5.0).  16 bits: the product m r is rounded in both directions (a
-// quotient 6.9 -> 7.2 us at 65536 x 128 bf16).
-template <class T> struct RowStat {
-    float mean, rstd, nm;
+// must be the same): xh from the difference, exact near the mean.  w and b come multiplied by the dropout factor
+// (a ReLU commutes with it).  The mean is a quotient: a product, sum (1 / N), goes into the difference unrounded
+// (one fma), and the forward's u is then not that of the stored mean; and a row of one value is off by its last bit
+// times rstd, up to 1 / sqrt(eps).  For 16-bit values too, whose rows often hold few different values (as x r - m r
+// with a product for m, constant rows of 5000 missed the bias by 0.1): 65536 x 128 bf16 forward 6.9 -> 7.2 us, 32768 x
+// 517 f16 backward 37.0 -> 38.3, elsewhere up to 1 %.
+struct RowStat {
+    float mean, rstd;
     MMVAE_DEV void set(float m, float r) {
         mean = m;
         rstd = r;
-        nm = -m * r;
     }
-    static MMVAE_DEV float mean_of(float sum, int N, float inv) { return sizeof(T) == 4 ? sum / (float)N : sum * inv; }
-    MMVAE_DEV float xh(float x) const { return sizeof(T) == 4 ? (x - mean) * rstd : __builtin_fmaf(x, rstd, nm); }
+    MMVAE_DEV float xh(float x) const { return (x - mean) * rstd; }
     MMVAE_DEV float u(float x, float w, float b) const { return __builtin_fmaf(xh(x), w, b); }
 };
 // 8 weights times the factor
@@ -144,7 +142,7 @@ __global__ __launch_bounds__(BLK) void k_ln_fwd(NormP a) {
             for (int i = 0; i < 8; ++i) t += xc[j].get(i);
             s += !EVEN || (j * TPR + lane) * 8 < N ? t : 0.f;
         }
-        const float mean = RowStat<T>::mean_of(row_sum<TPR>(s, red[0]), N, inv);
+        const float mean = row_sum<TPR>(s, red[0]) / (float)N;
         float q = 0.f;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
@@ -157,7 +155,7 @@ __global__ __launch_bounds__(BLK) void k_ln_fwd(NormP a) {
             }
             q += !EVEN || n > 0 ? t : 0.f;
         }
-        RowStat<T> st;
+        RowStat st;
         st.set(mean, 1.f / sqrtf(row_sum<TPR>(q, red[1]) * inv + a.eps));
         if (ok) {
             T* yr = (T*)a.y + row * a.ldy;
@@ -220,7 +218,7 @@ template <class T, bool MASK, bool EVEN> MMVAE_DEV void ln_strip(const NormP& a,
     const int64_t step = 64 * sw;
     for (int64_t r0 = (wave % sw) * 64 + lane; r0 < a.M && n > 0; r0 += 2 * step) {  // two rows at once
         Chunk<T> x[2], d[2];
-        RowStat<T> st[2];
+        RowStat st[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const int64_t row = r0 + step * k, rr = row < a.M ? row : r0;
@@ -345,7 +343,7 @@ __global__ __launch_bounds__(BLK, BLK / 256) void k_ln_bwd(NormP a) {
         } else {
             fetch(row, xc, dc, mean, rstd);
         }
-        RowStat<T> st;
+        RowStat st;
         st.set(mean, rstd);
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
@@ -526,7 +524,7 @@ template <class T> __global__ __launch_bounds__(1024) void k_ln_fwd_long(NormP a
             for (int i = 0; i < 8; ++i) t += c.get(i);
             s += t;
         }
-        const float mean = RowStat<T>::mean_of(row_sum<1024>(s, red[0]), N, inv);
+        const float mean = row_sum<1024>(s, red[0]) / (float)N;
         float q = 0.f;
         for (int64_t col = threadIdx.x * 8; col < N; col += 8192) {
             const int n = (int)(N - col);
@@ -539,7 +537,7 @@ template <class T> __global__ __launch_bounds__(1024) void k_ln_fwd_long(NormP a
             }
             q += t;
         }
-        RowStat<T> st;
+        RowStat st;
         st.set(mean, 1.f / sqrtf(row_sum<1024>(q, red[1]) * inv + a.eps));
         T* yr = (T*)a.y + row * a.ldy;
         for (int64_t col = threadIdx.x * 8; col < N; col += 8192) {
@@ -569,7 +567,7 @@ template <class T> __global__ __launch_bounds__(1024) void k_ln_fwd_long(NormP a
 }
 // one chunk's dy without what dropout and ReLU take away, xh, and the weights times the dropout factor
 template <class T>
-MMVAE_DEV void ln_du(const NormP& a, int64_t row, int64_t col, const RowStat<T>& st, float w[8], float du[8], float xh[8]) {
+MMVAE_DEV void ln_du(const NormP& a, int64_t row, int64_t col, const RowStat& st, float w[8], float du[8], float xh[8]) {
     const int n = (int)(a.N - col);
     const Chunk<T> xc = ld8((const T*)a.x + row * a.ldx + col, n), dc = ld8((const T*)a.dy + row * a.lddy + col, n);
     const float sc = a.drop.thr ? a.drop.s : 1.f;
@@ -592,7 +590,7 @@ template <class T> __global__ __launch_bounds__(1024) void k_ln_bwd_long(NormP a
     const float inv = 1.f / (float)a.N;
     drop_state(a.drop);
     for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
-        RowStat<T> st;
+        RowStat st;
         st.set(a.mean[row], a.rstd[row]);
         float s1 = 0.f, s2 = 0.f, w[8], du[8], xh[8];
         for (int64_t col = threadIdx.x * 8; col < a.N; col += 8192) {
@@ -625,7 +623,7 @@ template <class T> __global__ __launch_bounds__(256) void k_ln_cols(NormP a) {
     drop_state(a.drop);
     float aw[8] = {}, ab[8] = {}, w[8], du[8], xh[8];
     for (int64_t row = blockIdx.y; row < a.M; row += gridDim.y) {
-        RowStat<T> st;
+        RowStat st;
         st.set(a.mean[row], a.rstd[row]);
         ln_du<T>(a, row, col, st, w, du, xh);
 #pragma unroll

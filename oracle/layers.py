@@ -70,6 +70,7 @@ def norm_grads(dy, x, w, eps, factor, mask):
     dx = rstd * (g - c1 - xh * c2)
     # A row's sums are chains of at most ROW additions, so the mean is off by ROW u mean|x|, xh by
     # ROW u A with A = rstd mean|x| + |xh| + 1, and the means of g and g xh by ROW u of their absolute sums.
+    # (First order: for ROW u A well below 1, means up to some 10^4 times the spread.)
     a = rstd * x.abs().mean(1, keepdim=True) + xh.abs() + 1
     ag = (g.abs() * a).mean(1, keepdim=True)
     bdx = ROW * U32 * rstd * (2 * g.abs() + 2 * g.abs().mean(1, keepdim=True) + 2 * a * (g * xh).abs().mean(1, keepdim=True) + xh.abs() * 2 * ag)

@@ -185,14 +185,34 @@ def test_norm_relu_takes_one_side_in_both_directions(M, N, off, dtype):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("N", [7, 48, 500, 2049, 12000, 33000])
 def test_norm_of_constant_rows_is_the_bias(N, dtype):
-    """Rows of one value whose sum is exact in 32 bits: in f32 the mean is that value and y the bias."""
+    """Rows of one value whose sum is exact in 32 bits: the mean is that value and y the bias."""
     x = torch.tensor([1.0, -3.0, 0.5, 100.0, 0.0], device=DEV).to(dtype)[:, None].expand(5, N).contiguous()
     _, dy, w, b = make(5, N, dtype)
     y, mean, rstd = ops.layer_norm_forward(x, w, b)
-    if dtype == F32:
-        assert torch.equal(mean, x[:, 0]) and torch.equal(y, b.expand(5, N))
-    assert torch.equal(y[4], b.to(dtype))  # (16 bits: xh = x r - m r is off by the product's rounding where the row is not 0)
+    assert torch.equal(mean, x[:, 0].float()) and torch.equal(y, b.to(dtype).expand(5, N))
     check_norm(x, dy, w, b)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("off", [30.0, 1000.0, -5000.0])
+@pytest.mark.parametrize("M,N", [(40, 500), (600, 1000), (5, 16400), (3, 33000), (2500, 96)])
+def test_norm_of_rows_far_from_zero(M, N, off, dtype):
+    """Means far above the spread: in 16 bits such rows hold few different values, or one."""
+    x, dy, w, b = make(M, N, F32)
+    x, dy = (3 * x + off).to(dtype), dy.to(dtype)
+    check_norm(x, dy, w, b)
+    check_norm(x, dy, w, b, relu=True, p=0.25, seed=3)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_norm_of_rows_of_one_value_or_one_other(dtype):
+    x, dy, w, b = make(12, 4000, dtype)
+    x = x.clone()
+    for r, v in enumerate((3.3, 0.0, 60000.0, 1e-6, 0.1, 100.0)):
+        x[r] = v
+    x[4, 7], x[5, 9] = 0.2, 101.0
+    check_norm(x, dy, w, b)
+    check_norm(x, dy, w, b, eps=1e-12)
 
 
 def test_norm_infinities_stay_in_their_rows():
