@@ -14,10 +14,10 @@ namespace mmvae {
 // reads x and dy and writes dx; the row sums between a row's loads and its stores are hidden by
 // other rows' waves, or by the next row's loads where a row fills the workgroup.  Measured:
 //                       forward                backward
-//   32768 x 1024 bf16   29.6 us, 4.5 TB/s      44.0 us, 4.6 TB/s   (with dropout)
-//   4096 x 20000 bf16   67 us,   4.9 TB/s      123 us,  4.0 TB/s
-//   4096 x 128 f32      3.9 us                 4.7 us              (with dropout)
-//   100 x 48 f32        2.6 us                 3.2 us              (a launch's time)
+//   32768 x 1024 bf16   29.8 us, 4.5 TB/s      44.4 us, 4.5 TB/s   (with dropout)
+//   4096 x 20000 bf16   68 us,   4.8 TB/s      123 us,  4.0 TB/s
+//   4096 x 128 f32      4.2 us                 4.7 us              (with dropout)
+//   100 x 48 f32        2.7 us                 3.7 us              (a launch's time)
 // against 5.1 TB/s of a large copy.  The backward of long rows is the furthest off: its column sums
 // (16 registers a chunk) leave room for two rows in flight in 8 waves of a CU.
 // =======================================================================================
@@ -507,7 +507,7 @@ __global__ __launch_bounds__(1024) void k_ln_wred(int N, int64_t Np, int G, cons
 
 // Rows too long for the registers (N > 32,768): each sweep reads the row again, from the last-level cache
 // where it fits (2048 x 40000 bf16: forward 104 us, 3.1 TB/s of x and y; backward 235 us).  32768 / 32776 columns
-// of 4096 bf16 rows: forward 100 / 187 us, backward 264 / 385.
+// of 4096 bf16 rows: forward 102 / 187 us, backward 265 / 386.
 static constexpr int LONG_N = 32768;
 template <class T> __global__ __launch_bounds__(1024) void k_ln_fwd_long(NormP a) {
     __shared__ float red[2][16];
